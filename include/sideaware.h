@@ -149,6 +149,73 @@ sideaware_status_t sideaware_rope_precompute_freqs(float* freqs_cis, int dim, in
 sideaware_status_t sideaware_silu_mul_bf16(void* out, const void* a, const void* b, float scale,
                                            size_t n, int device, sideaware_stream_t stream);
 
+/* ---- operators of image and video models (no counterpart in the reference) ----
+ * Element types: 0 = fp32, 1 = bf16, 2 = fp16; arithmetic in fp32, one rounding at the end.  Plain launches on
+ * `stream`: nothing is kept from one call for the next, so calls may run at the same time on several streams and
+ * be recorded in CUDA graphs, as long as their outputs and workspaces are their own. */
+
+/* Rotary positions with several axes (time, height, width, ...), in place on packed [B, T, Nq + 2*Nkv, HS]: pair i of
+ * every Q and K head is turned by pos[axis(i)][b][t] * f(i).  V heads and the elements of a head behind the first
+ * 2*pairs are not touched.  Positions may be negative and need no table; the angle is exact however far they are. */
+#define SIDEAWARE_ROPE_MAX_AXES 8
+#define SIDEAWARE_ROPE_MAX_PAIRS 256
+typedef struct sideaware_rope_axes_t {
+    int B, T, Nq, Nkv, HS;
+    int pairs;          /* turned pairs of a head: entries of the spectrum, 2*pairs <= HS */
+    int axes;           /* leading dimension of the positions */
+    int layout;         /* 0: pair i = elements (2i, 2i+1); 1: elements (i, i + pairs) */
+    int dtype;
+    int position_dtype; /* 0 = int32, 1 = int64 */
+    long long stride_b, stride_t;                            /* of qkv, in elements; heads and their elements are dense */
+    long long pos_stride_axis, pos_stride_b, pos_stride_t;   /* of the positions, in elements; 0 = the same for all */
+} sideaware_rope_axes_t;
+/* Fills spectrum[pairs], 64-bit words in device memory: f(i) / 2 pi as a binary fraction of a turn, the axis in the low
+ * three bits.  pairs_per_axis: host memory.  arrangement 0 ("own"): every axis has a run of pairs and a spectrum of its
+ * own, f = theta^(-j / n) for the j-th of its n pairs; 1 ("shared"): one spectrum theta^(-i / pairs) over all pairs, each
+ * axis a run of it; 2 ("interleaved"): the same spectrum, its pairs dealt to the axes in turn while they have any left. */
+sideaware_status_t sideaware_rope_axes_spectrum(void* spectrum, const int* pairs_per_axis, int axes, double theta,
+                                                int arrangement, int device, sideaware_stream_t stream);
+sideaware_status_t sideaware_rope_axes_forward(void* qkv, const void* positions, const void* spectrum,
+                                               const sideaware_rope_axes_t* shape, int device, sideaware_stream_t stream);
+/* In place on the gradient of the packed tensor: the turn by the opposite angle. */
+sideaware_status_t sideaware_rope_axes_backward(void* dqkv, const void* positions, const void* spectrum,
+                                                const sideaware_rope_axes_t* shape, int device, sideaware_stream_t stream);
+
+/* Group norm with an optional SiLU on dense channels-last tensors [N, S, C] (S = all spatial positions); groups are
+ * C / G neighbouring channels.  mean and rstd [N, G] fp32 are written by the forward pass and read by the backward pass.
+ * weight and bias [C] (param_dtype) may each be NULL, as may dweight and dbias.  out may be x, dx may be dout or x.
+ * The same inputs give the same bits: no atomics. */
+typedef struct sideaware_group_norm_t {
+    long long S;
+    int N, C, G;
+    float eps;       /* forward only */
+    int silu;        /* 0: y = z, 1: y = z * sigmoid(z) */
+    int dtype;       /* of x, out and their gradients */
+    int param_dtype; /* of weight, bias and their gradients */
+} sideaware_group_norm_t;
+/* Bytes of device memory a call needs; it may be used again by the next call on the same stream.  0 = none (or, with an
+ * error recorded, an invalid shape). */
+size_t sideaware_group_norm_workspace(const sideaware_group_norm_t* shape, int backward);
+sideaware_status_t sideaware_group_norm_forward(void* out, float* mean, float* rstd, const void* x, const void* weight,
+                                                const void* bias, const sideaware_group_norm_t* shape, void* workspace,
+                                                size_t workspace_bytes, int device, sideaware_stream_t stream);
+sideaware_status_t sideaware_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x,
+                                                 const float* mean, const float* rstd, const void* weight, const void* bias,
+                                                 const sideaware_group_norm_t* shape, void* workspace, size_t workspace_bytes,
+                                                 int device, sideaware_stream_t stream);
+
+/* out = residual + (keep ? x / (1 - p) : 0); residual may be NULL.  A dropped element is 0 (or the residual) whatever x
+ * holds there.  The mask is never stored: element i is dropped when u_i < round(p 2^32), u_i being a 32-bit number from
+ * Philox4x32-10 with the key rng[0] and the counter (i / 8, rng[1]): 16 bits of block (i / 8, rng[1]), completed by the same
+ * 16 bits of block (2^63 + i / 8, rng[1]).  rng: two 64-bit words (seed, number of the call) in device memory, 16-byte
+ * aligned; every call of a model takes a number of its own, and the backward pass the forward pass's.  out may be x or
+ * the residual. */
+sideaware_status_t sideaware_dropout_forward(void* out, const void* x, const void* residual, const void* rng, double p,
+                                             size_t n, int dtype, int device, sideaware_stream_t stream);
+/* dx = keep ? dout / (1 - p) : 0 with the forward pass's rng (the residual's gradient is dout itself). */
+sideaware_status_t sideaware_dropout_backward(void* dx, const void* dout, const void* rng, double p, size_t n, int dtype,
+                                              int device, sideaware_stream_t stream);
+
 /* Compiles a functor header with NVRTC for sm_100a without loading it, so headers
  * can be checked on a machine without a GPU.  wide != 0 selects the 64-bit index
  * variant.  Returns 0 on success; the compiler log is copied to log_out.  A header that

@@ -27,6 +27,16 @@ class Stats(ctypes.Structure):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
 
 
+class RopeAxes(ctypes.Structure):
+    _fields_ = ([(n, c.c_int) for n in ("B", "T", "Nq", "Nkv", "HS", "pairs", "axes", "layout", "dtype", "position_dtype")]
+                + [(n, c.c_longlong) for n in ("stride_b", "stride_t", "pos_stride_axis", "pos_stride_b", "pos_stride_t")])
+
+
+class GroupNorm(ctypes.Structure):
+    _fields_ = [("S", c.c_longlong), ("N", c.c_int), ("C", c.c_int), ("G", c.c_int), ("eps", c.c_float), ("silu", c.c_int),
+                ("dtype", c.c_int), ("param_dtype", c.c_int)]
+
+
 # name -> (restype, argtypes); the complete exported surface
 SIGNATURES = {
     # reference-compatible entry points
@@ -64,6 +74,14 @@ SIGNATURES = {
     "sideaware_rope_backward": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sideaware_rope_precompute_freqs": (_i, [_vp, _i, _i, c.c_float, _i, _i, _vp]),
     "sideaware_silu_mul_bf16": (_i, [_vp, _vp, _vp, c.c_float, _sz, _i, _vp]),
+    "sideaware_rope_axes_spectrum": (_i, [_vp, c.POINTER(_i), _i, c.c_double, _i, _i, _vp]),
+    "sideaware_rope_axes_forward": (_i, [_vp, _vp, _vp, c.POINTER(RopeAxes), _i, _vp]),
+    "sideaware_rope_axes_backward": (_i, [_vp, _vp, _vp, c.POINTER(RopeAxes), _i, _vp]),
+    "sideaware_group_norm_workspace": (_sz, [c.POINTER(GroupNorm), _i]),
+    "sideaware_group_norm_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, c.POINTER(GroupNorm), _vp, _sz, _i, _vp]),
+    "sideaware_group_norm_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, c.POINTER(GroupNorm), _vp, _sz, _i, _vp]),
+    "sideaware_dropout_forward": (_i, [_vp, _vp, _vp, _vp, c.c_double, _sz, _i, _i, _vp]),
+    "sideaware_dropout_backward": (_i, [_vp, _vp, _vp, c.c_double, _sz, _i, _i, _vp]),
     "sideaware_compile_check": (_i, [c.c_char_p, _i, c.c_char_p, _sz]),
     "sideaware_set_placement": (None, [_i]),
     "sideaware_get_placement": (_i, []),

@@ -13,6 +13,19 @@ from . import _binding
 
 _state = {"sa": None}
 
+_ROPE_LAYOUTS = {"interleaved": 0, "halves": 1}
+_ROPE_ARRANGEMENTS = {"own": 0, "shared": 1, "interleaved": 2}
+_DTYPE_CODES = {}  # torch dtype -> element type of the C ABI; filled on first use, torch is imported late
+
+
+def _dtype_code(dtype) -> int:
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    code = _DTYPE_CODES.get(dtype)
+    assert code is not None, f"dtype must be float32, bfloat16 or float16, not {dtype}"
+    return code
+
 
 def _stream_ptr(stream) -> int:
     if stream is None:
@@ -266,6 +279,143 @@ class SideAware:
         # in which the functor skips that bookkeeping)
         self.elementwise(kid, out[:n], None, None, None, x, None, None, None, scales.view(torch.int32),
                          n // 8 if n % 32 else 0)
+
+    # -- operators of image and video models --------------------------------------
+    def _done(self, rc: int, what: str) -> None:
+        if rc != 0:
+            raise RuntimeError(f"{what} failed with CUDA error {rc}: {self.last_error()}")
+
+    def rope_axes_spectrum(self, pairs_per_axis, theta: float = 10000.0, arrangement: str = "own", device=None):
+        """The spectrum that rope_axes_forward / _backward read: int64 [sum(pairs_per_axis)], made on the GPU.
+        arrangement "own": every axis has a run of pairs and frequencies theta^(-j/n) of its own; "shared": one series
+        theta^(-i/pairs), each axis a run of it; "interleaved": the same series, its pairs dealt to the axes in turn."""
+        import torch
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        index = torch.cuda.current_device() if device.index is None else device.index
+        assert arrangement in _ROPE_ARRANGEMENTS, f"arrangement must be one of {sorted(_ROPE_ARRANGEMENTS)}"
+        pairs = [int(n) for n in pairs_per_axis]
+        assert 1 <= len(pairs) <= 8 and min(pairs) >= 0 and 1 <= sum(pairs) <= 256, "1 to 8 axes and 1 to 256 pairs over all of them"
+        spectrum = torch.empty(sum(pairs), dtype=torch.int64, device=device)
+        self._done(self.lib.sideaware_rope_axes_spectrum(
+            spectrum.data_ptr(), (ctypes.c_int * len(pairs))(*pairs), len(pairs), float(theta), _ROPE_ARRANGEMENTS[arrangement],
+            index, _stream_ptr(torch.cuda.current_stream(index))), "sideaware_rope_axes_spectrum")
+        return spectrum
+
+    def _rope_axes(self, call, what, qkv, positions, spectrum, n_q_heads, n_kv_heads, layout) -> None:
+        import torch
+        assert qkv.is_cuda and qkv.device == positions.device == spectrum.device, "all tensors must be on one CUDA device"
+        B, T, H, HS = qkv.shape
+        assert H == n_q_heads + 2 * n_kv_heads, "head dimension must hold q, k and v heads"
+        sb, st, sh, se = qkv.stride()
+        assert (se == 1 or HS == 1) and (sh == HS or H <= 1), "heads and their elements must be dense"
+        axes = positions.shape[0]
+        assert positions.dim() == 3 and tuple(positions.shape[1:]) == (B, T), "positions must be [axes, B, T]"
+        assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
+        assert spectrum.dim() == 1 and spectrum.dtype == torch.int64 and spectrum.is_contiguous(), "spectrum must be int64 [pairs]"
+        assert layout in _ROPE_LAYOUTS, f"layout must be one of {sorted(_ROPE_LAYOUTS)}"
+        shape = _binding.RopeAxes(B, T, n_q_heads, n_kv_heads, HS, spectrum.shape[0], axes, _ROPE_LAYOUTS[layout], _dtype_code(qkv.dtype),
+                                  1 if positions.dtype == torch.int64 else 0, sb, st, *positions.stride())
+        self._done(call(qkv.data_ptr(), positions.data_ptr(), spectrum.data_ptr(), ctypes.byref(shape), qkv.device.index,
+                        _stream_ptr(torch.cuda.current_stream(qkv.device))), what)
+
+    def rope_axes_forward(self, qkv, positions, spectrum, n_q_heads: int, n_kv_heads: int, layout: str = "interleaved") -> None:
+        """Rotary positions with several axes, in place on packed [B, T, Nq + 2 Nkv, HS] (fp32, bf16 or fp16; any strides
+        over B and T): pair i of every q and k head turns by positions[axis of i, b, t] times its frequency.
+        positions: int32 or int64 [axes, B, T], any strides and values; spectrum: rope_axes_spectrum.  A head of which the
+        spectrum's pairs fill only a part keeps its remaining elements.  layout: pair i = elements (2i, 2i + 1)
+        ("interleaved") or (i, i + pairs) ("halves")."""
+        self._rope_axes(self.lib.sideaware_rope_axes_forward, "sideaware_rope_axes_forward", qkv, positions, spectrum,
+                        n_q_heads, n_kv_heads, layout)
+
+    def rope_axes_backward(self, dqkv, positions, spectrum, n_q_heads: int, n_kv_heads: int, layout: str = "interleaved") -> None:
+        """In place on the gradient of the packed tensor: the turn by the opposite angle."""
+        self._rope_axes(self.lib.sideaware_rope_axes_backward, "sideaware_rope_axes_backward", dqkv, positions, spectrum,
+                        n_q_heads, n_kv_heads, layout)
+
+    def _group_norm_shape(self, x, groups, eps, silu, like, params):
+        """Checks what forward and backward share; returns the shape for the C ABI.  `like`: tensors shaped as x;
+        `params`: tensors of C entries, or None."""
+        assert x.is_cuda and x.is_contiguous() and x.dim() >= 2, "x must be a dense CUDA tensor [N, ..., C]"
+        N, C = x.shape[0], x.shape[-1]
+        assert groups >= 1 and C >= 1 and C % groups == 0, "the channels must divide evenly into the groups"
+        for t in like:
+            assert t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device, \
+                "out, dx and dout must be dense tensors of x's shape, dtype and device"
+        param_dtype = None
+        for t in params:
+            if t is not None:
+                assert t.numel() == C and t.is_contiguous() and t.device == x.device, "weight, bias and their gradients must be dense [C]"
+                assert param_dtype is None or t.dtype == param_dtype, "weight, bias and their gradients must have one dtype"
+                param_dtype = t.dtype
+        S = 1
+        for n in x.shape[1:-1]:
+            S *= n
+        return _binding.GroupNorm(S, N, C, groups, eps, 1 if silu else 0, _dtype_code(x.dtype),
+                                  0 if param_dtype is None else _dtype_code(param_dtype))
+
+    def _group_norm_workspace(self, shape, backward, device):
+        import torch
+        before = self.error_count()
+        size = self.lib.sideaware_group_norm_workspace(ctypes.byref(shape), backward)
+        self._checked(before, "sideaware_group_norm_workspace")
+        return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+    def group_norm_forward(self, out, mean, rstd, x, weight, bias, groups: int, eps: float = 1e-5, silu: bool = True) -> None:
+        """Group norm, then SiLU unless silu is False, on dense channels-last x [N, ..., C] (fp32, bf16 or fp16; a
+        channels_last [N, C, H, W] tensor is passed as x.permute(0, 2, 3, 1)).  out: like x, may be x.  mean and rstd:
+        fp32 [N, groups], written for the backward pass.  weight, bias: [C] of one dtype, each may be None."""
+        import torch
+        shape = self._group_norm_shape(x, groups, eps, silu, (out,), (weight, bias))
+        for t in (mean, rstd):
+            assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == shape.N * groups and t.device == x.device, \
+                "mean and rstd must be dense fp32 [N, groups]"
+        workspace, size = self._group_norm_workspace(shape, 0, x.device)
+        self._done(self.lib.sideaware_group_norm_forward(
+            out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x.data_ptr(), weight.data_ptr() if weight is not None else 0,
+            bias.data_ptr() if bias is not None else 0, ctypes.byref(shape), workspace.data_ptr() if size else 0, size,
+            x.device.index, _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_group_norm_forward")
+
+    def group_norm_backward(self, dx, dweight, dbias, dout, x, mean, rstd, weight, bias, groups: int, silu: bool = True) -> None:
+        """Gradients of group_norm_forward: dx like x (may be dout or x), dweight and dbias [C] like weight and bias, each
+        may be None.  mean and rstd: the forward pass's."""
+        import torch
+        shape = self._group_norm_shape(x, groups, 0.0, silu, (dx, dout), (weight, bias, dweight, dbias))
+        for t in (mean, rstd):
+            assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == shape.N * groups and t.device == x.device, \
+                "mean and rstd must be dense fp32 [N, groups]"
+        workspace, size = self._group_norm_workspace(shape, 1, x.device)
+        ptr = [t.data_ptr() if t is not None else 0 for t in (dx, dweight, dbias, dout, x, mean, rstd, weight, bias)]
+        self._done(self.lib.sideaware_group_norm_backward(
+            *ptr, ctypes.byref(shape), workspace.data_ptr() if size else 0, size, x.device.index,
+            _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_group_norm_backward")
+
+    def _dropout_check(self, out, x, rng, residual) -> None:
+        import torch
+        assert x.is_cuda and x.is_contiguous(), "x must be a dense CUDA tensor"
+        for t in (out, residual):
+            assert t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device), \
+                "out and residual must be dense tensors of x's shape, dtype and device"
+        assert rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous() and rng.device == x.device, \
+            "rng must be int64 (seed, number of the call) on x's device"
+
+    def dropout_forward(self, out, x, rng, p: float, residual=None) -> None:
+        """out = residual + (keep ? x / (1 - p) : 0) (fp32, bf16 or fp16; out may be x or residual).  The mask is drawn
+        from rng, an int64 CUDA tensor (seed, number of the call): every call of a model takes a number of its own, and
+        dropout_backward the forward pass's pair.  The pair is read on the device, so a replayed CUDA graph that advances
+        it draws new masks."""
+        import torch
+        self._dropout_check(out, x, rng, residual)
+        self._done(self.lib.sideaware_dropout_forward(
+            out.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else 0, rng.data_ptr(), p, x.numel(),
+            _dtype_code(x.dtype), x.device.index, _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_dropout_forward")
+
+    def dropout_backward(self, dx, dout, rng, p: float) -> None:
+        """dx = keep ? dout / (1 - p) : 0 with the forward pass's rng (the residual's gradient is dout itself)."""
+        import torch
+        self._dropout_check(dx, dout, rng, None)
+        self._done(self.lib.sideaware_dropout_backward(
+            dx.data_ptr(), dout.data_ptr(), rng.data_ptr(), p, dout.numel(), _dtype_code(dout.dtype), dout.device.index,
+            _stream_ptr(torch.cuda.current_stream(dout.device))), "sideaware_dropout_backward")
 
     def side_index_tensor(self):
         import torch

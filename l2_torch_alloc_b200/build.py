@@ -23,7 +23,8 @@ OUT = os.path.join(HERE, "sideaware.so")
 OUT_ALLOC = os.path.join(HERE, "sideaware_alloc.so")
 
 SOURCES = ["sa_api.cpp", "sa_context.cpp", "sa_alloc.cpp", "sa_driver.cpp", "sa_jit.cpp", "sa_topology.cpp",
-           "sa_probe.cu", "sa_kernels.cu", "sa_memcpy_bulk.cu", "sa_rope_bulk.cu"]
+           "sa_probe.cu", "sa_kernels.cu", "sa_memcpy_bulk.cu", "sa_rope_bulk.cu",
+           "sa_ops_api.cpp", "sa_rope_axes.cu", "sa_group_norm.cu", "sa_dropout.cu"]
 ALLOC_ONLY_SOURCES = ["sa_api.cpp", "sa_context.cpp", "sa_alloc.cpp", "sa_driver.cpp", "sa_topology.cpp", "sa_probe.cu"]
 EMBEDDED = [("kSaSchedSource", "sa_sched.cuh"), ("kSaJitTemplateSource", "sa_jit_template.cuh")]
 

@@ -1,5 +1,5 @@
 """torch.ops.sideaware.* registration (the custom ops of test.py:147-157, plus rope_forward,
-rope_backward, rope_freqs and silu_mul).  Kept in a module of its own WITHOUT postponed annotation evaluation:
+rope_backward, rope_freqs, silu_mul and the operators of image and video models).  Kept in a module of its own WITHOUT postponed annotation evaluation:
 torch.library.infer_schema reads the real annotation objects."""
 from typing import Optional
 
@@ -39,6 +39,29 @@ def register(sa) -> None:
     def silu_mul(out: Tensor, a: Tensor, b: Tensor, scale: float) -> None:
         sa.silu_mul(out, a, b, scale)
 
+    def rope_axes_forward(qkv: Tensor, positions: Tensor, spectrum: Tensor, n_q_heads: int, n_kv_heads: int,
+                          layout: str = "interleaved") -> None:
+        sa.rope_axes_forward(qkv, positions, spectrum, n_q_heads, n_kv_heads, layout)
+
+    def rope_axes_backward(dqkv: Tensor, positions: Tensor, spectrum: Tensor, n_q_heads: int, n_kv_heads: int,
+                           layout: str = "interleaved") -> None:
+        sa.rope_axes_backward(dqkv, positions, spectrum, n_q_heads, n_kv_heads, layout)
+
+    def group_norm_forward(out: Tensor, mean: Tensor, rstd: Tensor, x: Tensor, weight: Optional[Tensor],
+                           bias: Optional[Tensor], groups: int, eps: float = 1e-5, silu: bool = True) -> None:
+        sa.group_norm_forward(out, mean, rstd, x, weight, bias, groups, eps, silu)
+
+    def group_norm_backward(dx: Tensor, dweight: Optional[Tensor], dbias: Optional[Tensor], dout: Tensor, x: Tensor,
+                            mean: Tensor, rstd: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int,
+                            silu: bool = True) -> None:
+        sa.group_norm_backward(dx, dweight, dbias, dout, x, mean, rstd, weight, bias, groups, silu)
+
+    def dropout_forward(out: Tensor, x: Tensor, rng: Tensor, p: float, residual: Optional[Tensor] = None) -> None:
+        sa.dropout_forward(out, x, rng, p, residual)
+
+    def dropout_backward(dx: Tensor, dout: Tensor, rng: Tensor, p: float) -> None:
+        sa.dropout_backward(dx, dout, rng, p)
+
     lib = torch.library.Library("sideaware", "FRAGMENT")
 
     def reg(name, fn, mutates):
@@ -53,4 +76,10 @@ def register(sa) -> None:
     reg("rope_backward", rope_backward, ["dqkv"])
     reg("rope_freqs", rope_freqs, ["freqs_cis"])
     reg("silu_mul", silu_mul, ["out"])
+    reg("rope_axes_forward", rope_axes_forward, ["qkv"])
+    reg("rope_axes_backward", rope_axes_backward, ["dqkv"])
+    reg("group_norm_forward", group_norm_forward, ["out", "mean", "rstd"])
+    reg("group_norm_backward", group_norm_backward, ["dx", "dweight", "dbias"])
+    reg("dropout_forward", dropout_forward, ["out"])
+    reg("dropout_backward", dropout_backward, ["dx"])
     _registered["lib"] = lib

@@ -366,13 +366,6 @@ sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __r
 // ---------------------------------------------------------------------------
 // resident: a cluster for a slab of groups of one sample
 // ---------------------------------------------------------------------------
-// Division by a launch constant: exact for n * d < 2^32 (n * (2^32 / d + 1) overshoots n / d * 2^32 by at most n).
-struct Divisor {
-    uint32_t d, m;
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1u ? n : __umulhi(n, m); }
-};
-Divisor divisor(uint32_t d) { return Divisor{d, d > 1 ? (uint32_t)(0x100000000ull / d + 1) : 0u}; }
-
 struct Slab {
     Norm p;
     int groups, width;     // groups of a slab, its channels = groups * D, a whole number of words
@@ -453,63 +446,6 @@ __device__ __forceinline__ void as_rows_arrive(int rows, F&& f) {
     f(stage_end(rows, 2), rows);
 }
 
-// Two fp32 numbers that one instruction works on (sm_100a: add, mul and fma .f32x2, each half rounded as usual).
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float x, float y) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ F2 negative(F2 a) { return F2{a.v ^ 0x8000000080000000ull}; }
-
-// elements 2k and 2k + 1 of a word (a word of one element: the second half is 0)
-template <class T, int V>
-__device__ __forceinline__ F2 pair_of(const SaVec<T, V>& v, int k) {
-    if constexpr (V == 1) {
-        return f2(sa_to_float(v.e[0]), 0.0f);
-    } else if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[k];
-        return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    } else if constexpr (sizeof(T) == 2) {
-        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&v)[k]);
-        return f2(f.x, f.y);
-    } else {
-        return f2(v.e[2 * k], v.e[2 * k + 1]);
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void set_pair(SaVec<T, V>& v, int k, F2 a) {
-    float x, y;
-    split(a, x, y);
-    if constexpr (V == 1) {
-        v.e[0] = sa_from_float<T>(x);
-    } else if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
-        reinterpret_cast<__nv_bfloat162*>(&v)[k] = __floats2bfloat162_rn(x, y);
-    } else if constexpr (sizeof(T) == 2) {
-        reinterpret_cast<__half2*>(&v)[k] = __floats2half2_rn(x, y);
-    } else {
-        v.e[2 * k] = x;
-        v.e[2 * k + 1] = y;
-    }
-}
 // V floats of shared memory as pairs
 template <int V>
 __device__ __forceinline__ void shared_pairs(F2 (&out)[(V + 1) / 2], const float* p) {

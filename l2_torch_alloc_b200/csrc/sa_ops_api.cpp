@@ -61,6 +61,7 @@ cudaError_t rope_axes(const char* what, void* qkv, const void* positions, const 
         return refuse(what, "a pointer is not aligned to its elements");
     // tokens must not share memory: a row is `row` elements, rows of one index lie inside a step of the other
     const long long row = heads * sh->HS;
+    if (row > (1ll << 30)) return refuse(what, "more than 2^30 elements of a row");
     const long long sb = sh->stride_b, st = sh->stride_t;
     if ((sh->T > 1 && (st < row || st > (1ll << 40))) || (sh->B > 1 && (sb < row || sb > (1ll << 46)))) return refuse(what, "a stride of qkv is shorter than a row (or absurdly long)");
     if (sh->T > 1 && sh->B > 1 && sb < (sh->T - 1) * st + row && st < (sh->B - 1) * sb + row)

@@ -15,11 +15,13 @@
 
 namespace {
 
+constexpr uint32_t kMostThreads = 512;
+
 struct Shape {
     uint32_t tokens, T;               // B * T tokens
     uint32_t heads, head_groups;      // Nq + Nkv; threads of a token and a place = ceil(heads / heads per thread)
-    uint32_t slots;                   // places: words (interleaved) or pairs of words (halves) of a head
-    uint32_t per_token;               // threads of a token
+    Divisor by_slots;                 // places: words (interleaved) or pairs of words (halves) of a head
+    Divisor by_token;                 // threads of a token
     uint32_t tokens_per_block;
     uint32_t axes;
     int HS, pairs;
@@ -62,82 +64,115 @@ struct Words {
     __device__ __forceinline__ T& operator[](int i) { return w[i / W].e[i % W]; }
 };
 
+// (x, y) -> (x cos - y sin, x sin + y cos) for two pairs at once
+__device__ __forceinline__ void turn(F2& x, F2& y, F2 c, F2 s) {
+    const F2 a = fma2(x, c, negative(y * s));
+    y = fma2(x, s, y * c);
+    x = a;
+}
 template <class T>
-__device__ __forceinline__ void turn(T& a, T& b, float c, float s) {
-    const float x = sa_to_float(a), y = sa_to_float(b);
-    a = sa_from_float<T>(fmaf(x, c, -(y * s)));
-    b = sa_from_float<T>(fmaf(x, s, y * c));
+__device__ __forceinline__ void turn(T& xa, T& ya, T& xb, T& yb, F2 c, F2 s) {
+    F2 x = f2(sa_to_float(xa), sa_to_float(xb)), y = f2(sa_to_float(ya), sa_to_float(yb));
+    turn(x, y, c, s);
+    float p, q;
+    split(x, p, q);
+    xa = sa_from_float<T>(p);
+    xb = sa_from_float<T>(q);
+    split(y, p, q);
+    ya = sa_from_float<T>(p);
+    yb = sa_from_float<T>(q);
 }
 
 // HALVES: pair i = elements (i, i + pairs), a thread has two words of V elements (V pairs) of each of U heads;
 // else pair i = elements (2 i, 2 i + 1), one word of V elements (V / 2 pairs) of each of U heads.
 template <class T, int V, int W, bool HALVES, int U>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(kMostThreads, 2)
 sa_rope_axes_kernel(T* __restrict__ x, const void* __restrict__ positions, const unsigned long long* __restrict__ spectrum,
                     const __grid_constant__ Shape sh) {
     constexpr int kPairs = HALVES ? V : V / 2;
     constexpr int kParts = HALVES ? 2 : 1;
     const uint32_t local = blockIdx.y * blockDim.x + threadIdx.x;
-    const uint32_t in_block = local / sh.per_token, unit = local - in_block * sh.per_token;
+    const uint32_t in_block = sh.tokens_per_block > 1 ? sh.by_token.div(local) : local >= sh.by_token.d ? 1u : 0u;
+    const uint32_t unit = local - in_block * sh.by_token.d;
     const uint32_t token = blockIdx.x * sh.tokens_per_block + in_block;
     if (in_block >= sh.tokens_per_block || token >= sh.tokens) return;
-    const uint32_t hg = unit / sh.slots, slot = unit - hg * sh.slots;
-    const uint32_t b = token / sh.T, t = token - b * sh.T;
-    T* const row = x + b * sh.stride_b + t * sh.stride_t + slot * V;
+    const uint32_t hg = sh.by_slots.div(unit), slot = unit - hg * sh.by_slots.d;
+    const uint32_t b = token < sh.T ? 0u : token / sh.T, t = token - b * sh.T;
+    T* const row = x + b * sh.stride_b + t * sh.stride_t + slot * V + hg * (uint32_t)sh.HS;
+    const uint32_t step = sh.head_groups * (uint32_t)sh.HS; // from one of this thread's heads to the next
 
     Words<T, V, W> v[U][kParts];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const uint32_t h = hg + u * sh.head_groups;
-        if (h < sh.heads) {
+        if (hg + u * sh.head_groups < sh.heads) {
 #pragma unroll
-            for (int k = 0; k < kParts; ++k) v[u][k].load(row + (long long)h * sh.HS + k * sh.pairs);
+            for (int k = 0; k < kParts; ++k) v[u][k].load(row + u * step + k * sh.pairs);
         }
     }
     float c[kPairs], s[kPairs];
     const long long place = b * sh.pos_stride_b + t * sh.pos_stride_t;
+    uint32_t have = 0xffffffffu; // neighbouring pairs mostly share their axis
+    long long pos = 0;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
         const unsigned long long f = __ldg(spectrum + slot * kPairs + i);
         const uint32_t axis = min((uint32_t)f & 7u, sh.axes - 1u);
-        const long long at = place + axis * sh.pos_stride_axis;
-        const long long pos = sh.wide_positions ? __ldg(static_cast<const long long*>(positions) + at)
-                                                : (long long)__ldg(static_cast<const int*>(positions) + at);
+        if (axis != have) {
+            const long long at = place + axis * sh.pos_stride_axis;
+            pos = sh.wide_positions ? __ldg(static_cast<const long long*>(positions) + at)
+                                    : (long long)__ldg(static_cast<const int*>(positions) + at);
+            have = axis;
+        }
         const unsigned long long product = (unsigned long long)pos * (f & ~7ull);
         cos_sin_of_turn((uint32_t)(product >> 32), c[i], s[i]);
         if (sh.inverse) s[i] = -s[i];
     }
+    if constexpr (HALVES && V > 1) { // two neighbouring pairs of a head at a time
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t h = hg + u * sh.head_groups;
-        if (h < sh.heads) {
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2)
+                turn(v[u][0][i], v[u][1][i], v[u][0][i + 1], v[u][1][i + 1], f2(c[i], c[i + 1]), f2(s[i], s[i + 1]));
+        }
+    } else { // the same pair of two heads at a time
+#pragma unroll
+        for (int u = 0; u < U; u += 2) {
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-                if (HALVES) turn(v[u][0][i], v[u][kParts - 1][i], c[i], s[i]);
-                else turn(v[u][0][2 * i], v[u][0][2 * i + 1], c[i], s[i]);
+                constexpr int y = HALVES ? kParts - 1 : 0;
+                const int xi = HALVES ? i : 2 * i, yi = HALVES ? i : 2 * i + 1;
+                turn(v[u][0][xi], v[u][y][yi], v[u + 1][0][xi], v[u + 1][y][yi], f2(c[i], c[i]), f2(s[i], s[i]));
             }
+        }
+    }
 #pragma unroll
-            for (int k = 0; k < kParts; ++k) v[u][k].store(row + (long long)h * sh.HS + k * sh.pairs);
+    for (int u = 0; u < U; ++u) {
+        if (hg + u * sh.head_groups < sh.heads) {
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) v[u][k].store(row + u * step + k * sh.pairs);
         }
     }
 }
 
 template <class T, int V, int W, bool HALVES>
 cudaError_t launch(void* qkv, const void* positions, const void* spectrum, Shape s, cudaStream_t stream) {
-    constexpr int U = HALVES ? 2 : 4;
-    s.slots = (uint32_t)(HALVES ? s.pairs / V : 2 * s.pairs / V);
+    constexpr int U = V * (int)sizeof(T) == 16 && HALVES ? 2 : 4; // 64 bytes of each thread are in flight, 32 of narrow words
+    const uint32_t slots = (uint32_t)(HALVES ? s.pairs / V : 2 * s.pairs / V);
     s.head_groups = (s.heads + U - 1) / U;
-    const uint64_t per_token = (uint64_t)s.slots * s.head_groups;
-    if (per_token > (1u << 24)) return cudaErrorInvalidValue;
-    s.per_token = (uint32_t)per_token;
-    uint32_t threads = 512, rows = 1; // blocks of up to 512 threads: whole tokens, or a part of one
-    if (s.per_token <= 512) {
-        s.tokens_per_block = 512 / s.per_token;
-        threads = (s.tokens_per_block * s.per_token + 31) / 32 * 32;
+    const uint64_t most = (uint64_t)slots * s.head_groups;
+    if (most > (1u << 20)) return cudaErrorInvalidValue;
+    const uint32_t per_token = (uint32_t)most;
+    s.by_slots = divisor(slots);
+    s.by_token = divisor(per_token);
+    uint32_t threads, rows = 1; // blocks of 256 threads or a little more: whole tokens, or a part of one
+    if (per_token <= kMostThreads) {
+        s.tokens_per_block = (256 + per_token - 1) / per_token;
+        if (s.tokens_per_block * per_token > kMostThreads) s.tokens_per_block = 1;
+        threads = (s.tokens_per_block * per_token + 31) / 32 * 32;
     } else {
         s.tokens_per_block = 1;
-        rows = (s.per_token + 511) / 512;
-        threads = ((s.per_token + rows - 1) / rows + 31) / 32 * 32;
+        rows = (per_token + 255) / 256;
+        threads = ((per_token + rows - 1) / rows + 31) / 32 * 32;
     }
     const uint32_t blocks = (s.tokens + s.tokens_per_block - 1) / s.tokens_per_block;
     sa_rope_axes_kernel<T, V, W, HALVES, U><<<dim3(blocks, rows), threads, 0, stream>>>(

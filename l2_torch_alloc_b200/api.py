@@ -18,6 +18,12 @@ _ROPE_ARRANGEMENTS = {"own": 0, "shared": 1, "interleaved": 2}
 _DTYPE_CODES = {}  # torch dtype -> element type of the C ABI; filled on first use, torch is imported late
 
 
+def _current_stream(index: int) -> int:
+    """The current stream of a device as a pointer (torch.cuda.current_stream without the Stream object: 0.1 us, not 3)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _dtype_code(dtype) -> int:
     if not _DTYPE_CODES:
         import torch
@@ -43,6 +49,7 @@ class SideAware:
     def __init__(self, path: Optional[str] = None):
         self.lib = _binding.load(path)
         self.path = self.lib._path
+        self._norm_shapes = {}  # shape and types -> what the C ABI is told of them, and the workspace's size
 
     # -- errors ---------------------------------------------------------------
     def last_error(self) -> str:
@@ -298,12 +305,13 @@ class SideAware:
         spectrum = torch.empty(sum(pairs), dtype=torch.int64, device=device)
         self._done(self.lib.sideaware_rope_axes_spectrum(
             spectrum.data_ptr(), (ctypes.c_int * len(pairs))(*pairs), len(pairs), float(theta), _ROPE_ARRANGEMENTS[arrangement],
-            index, _stream_ptr(torch.cuda.current_stream(index))), "sideaware_rope_axes_spectrum")
+            index, _current_stream(index)), "sideaware_rope_axes_spectrum")
         return spectrum
 
     def _rope_axes(self, call, what, qkv, positions, spectrum, n_q_heads, n_kv_heads, layout) -> None:
         import torch
-        assert qkv.is_cuda and qkv.device == positions.device == spectrum.device, "all tensors must be on one CUDA device"
+        device = qkv.get_device()
+        assert device >= 0 and positions.get_device() == device and spectrum.get_device() == device, "all tensors must be on one CUDA device"
         B, T, H, HS = qkv.shape
         assert H == n_q_heads + 2 * n_kv_heads, "head dimension must hold q, k and v heads"
         sb, st, sh, se = qkv.stride()
@@ -315,8 +323,7 @@ class SideAware:
         assert layout in _ROPE_LAYOUTS, f"layout must be one of {sorted(_ROPE_LAYOUTS)}"
         shape = _binding.RopeAxes(B, T, n_q_heads, n_kv_heads, HS, spectrum.shape[0], axes, _ROPE_LAYOUTS[layout], _dtype_code(qkv.dtype),
                                   1 if positions.dtype == torch.int64 else 0, sb, st, *positions.stride())
-        self._done(call(qkv.data_ptr(), positions.data_ptr(), spectrum.data_ptr(), ctypes.byref(shape), qkv.device.index,
-                        _stream_ptr(torch.cuda.current_stream(qkv.device))), what)
+        self._done(call(qkv.data_ptr(), positions.data_ptr(), spectrum.data_ptr(), ctypes.byref(shape), device, _current_stream(device)), what)
 
     def rope_axes_forward(self, qkv, positions, spectrum, n_q_heads: int, n_kv_heads: int, layout: str = "interleaved") -> None:
         """Rotary positions with several axes, in place on packed [B, T, Nq + 2 Nkv, HS] (fp32, bf16 or fp16; any strides
@@ -332,90 +339,92 @@ class SideAware:
         self._rope_axes(self.lib.sideaware_rope_axes_backward, "sideaware_rope_axes_backward", dqkv, positions, spectrum,
                         n_q_heads, n_kv_heads, layout)
 
-    def _group_norm_shape(self, x, groups, eps, silu, like, params):
-        """Checks what forward and backward share; returns the shape for the C ABI.  `like`: tensors shaped as x;
-        `params`: tensors of C entries, or None."""
-        assert x.is_cuda and x.is_contiguous() and x.dim() >= 2, "x must be a dense CUDA tensor [N, ..., C]"
-        N, C = x.shape[0], x.shape[-1]
-        assert groups >= 1 and C >= 1 and C % groups == 0, "the channels must divide evenly into the groups"
+    def _group_norm_shape(self, x, groups, eps, silu, backward, like, stats, params):
+        """Checks what forward and backward share; returns (shape for the C ABI, workspace, its size).  `like`: tensors shaped
+        as x; `stats`: fp32 [N, groups]; `params`: tensors of C entries, or None."""
+        import torch
+        device = x.get_device()
+        assert device >= 0 and x.is_contiguous() and x.dim() >= 2, "x must be a dense CUDA tensor [N, ..., C]"
+        size, dtype = x.shape, x.dtype
+        N, C = size[0], size[-1]
         for t in like:
-            assert t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device, \
+            assert t.shape == size and t.dtype is dtype and t.is_contiguous() and t.get_device() == device, \
                 "out, dx and dout must be dense tensors of x's shape, dtype and device"
+        for t in stats:
+            assert t.dtype is torch.float32 and t.is_contiguous() and t.numel() == N * groups and t.get_device() == device, \
+                "mean and rstd must be dense fp32 [N, groups]"
         param_dtype = None
         for t in params:
             if t is not None:
-                assert t.numel() == C and t.is_contiguous() and t.device == x.device, "weight, bias and their gradients must be dense [C]"
-                assert param_dtype is None or t.dtype == param_dtype, "weight, bias and their gradients must have one dtype"
+                assert t.numel() == C and t.is_contiguous() and t.get_device() == device, "weight, bias and their gradients must be dense [C]"
+                assert param_dtype is None or t.dtype is param_dtype, "weight, bias and their gradients must have one dtype"
                 param_dtype = t.dtype
-        S = 1
-        for n in x.shape[1:-1]:
-            S *= n
-        return _binding.GroupNorm(S, N, C, groups, eps, 1 if silu else 0, _dtype_code(x.dtype),
-                                  0 if param_dtype is None else _dtype_code(param_dtype))
-
-    def _group_norm_workspace(self, shape, backward, device):
-        import torch
-        before = self.error_count()
-        size = self.lib.sideaware_group_norm_workspace(ctypes.byref(shape), backward)
-        self._checked(before, "sideaware_group_norm_workspace")
-        return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+        key = (size, dtype, groups, eps, silu, backward, param_dtype)
+        known = self._norm_shapes.get(key)
+        if known is None:
+            assert groups >= 1 and C >= 1 and C % groups == 0, "the channels must divide evenly into the groups"
+            S = 1
+            for n in size[1:-1]:
+                S *= n
+            shape = _binding.GroupNorm(S, N, C, groups, eps, 1 if silu else 0, _dtype_code(dtype),
+                                       0 if param_dtype is None else _dtype_code(param_dtype))
+            before = self.error_count()
+            need = self.lib.sideaware_group_norm_workspace(ctypes.byref(shape), backward)
+            self._checked(before, "sideaware_group_norm_workspace")
+            if len(self._norm_shapes) >= 256:  # a program whose shapes never come back
+                self._norm_shapes.clear()
+            known = self._norm_shapes[key] = (shape, need)
+        shape, need = known
+        return shape, (torch.empty(need, dtype=torch.uint8, device=x.device) if need else None), need
 
     def group_norm_forward(self, out, mean, rstd, x, weight, bias, groups: int, eps: float = 1e-5, silu: bool = True) -> None:
         """Group norm, then SiLU unless silu is False, on dense channels-last x [N, ..., C] (fp32, bf16 or fp16; a
         channels_last [N, C, H, W] tensor is passed as x.permute(0, 2, 3, 1)).  out: like x, may be x.  mean and rstd:
         fp32 [N, groups], written for the backward pass.  weight, bias: [C] of one dtype, each may be None."""
-        import torch
-        shape = self._group_norm_shape(x, groups, eps, silu, (out,), (weight, bias))
-        for t in (mean, rstd):
-            assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == shape.N * groups and t.device == x.device, \
-                "mean and rstd must be dense fp32 [N, groups]"
-        workspace, size = self._group_norm_workspace(shape, 0, x.device)
+        shape, workspace, size = self._group_norm_shape(x, groups, eps, silu, 0, (out,), (mean, rstd), (weight, bias))
+        device = x.get_device()
         self._done(self.lib.sideaware_group_norm_forward(
             out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x.data_ptr(), weight.data_ptr() if weight is not None else 0,
             bias.data_ptr() if bias is not None else 0, ctypes.byref(shape), workspace.data_ptr() if size else 0, size,
-            x.device.index, _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_group_norm_forward")
+            device, _current_stream(device)), "sideaware_group_norm_forward")
 
     def group_norm_backward(self, dx, dweight, dbias, dout, x, mean, rstd, weight, bias, groups: int, silu: bool = True) -> None:
         """Gradients of group_norm_forward: dx like x (may be dout or x), dweight and dbias [C] like weight and bias, each
         may be None.  mean and rstd: the forward pass's."""
-        import torch
-        shape = self._group_norm_shape(x, groups, 0.0, silu, (dx, dout), (weight, bias, dweight, dbias))
-        for t in (mean, rstd):
-            assert t.dtype == torch.float32 and t.is_contiguous() and t.numel() == shape.N * groups and t.device == x.device, \
-                "mean and rstd must be dense fp32 [N, groups]"
-        workspace, size = self._group_norm_workspace(shape, 1, x.device)
+        shape, workspace, size = self._group_norm_shape(x, groups, 0.0, silu, 1, (dx, dout), (mean, rstd), (weight, bias, dweight, dbias))
+        device = x.get_device()
         ptr = [t.data_ptr() if t is not None else 0 for t in (dx, dweight, dbias, dout, x, mean, rstd, weight, bias)]
         self._done(self.lib.sideaware_group_norm_backward(
-            *ptr, ctypes.byref(shape), workspace.data_ptr() if size else 0, size, x.device.index,
-            _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_group_norm_backward")
+            *ptr, ctypes.byref(shape), workspace.data_ptr() if size else 0, size, device, _current_stream(device)),
+            "sideaware_group_norm_backward")
 
-    def _dropout_check(self, out, x, rng, residual) -> None:
+    def _dropout_check(self, out, x, rng, residual) -> int:
         import torch
-        assert x.is_cuda and x.is_contiguous(), "x must be a dense CUDA tensor"
+        device = x.get_device()
+        assert device >= 0 and x.is_contiguous(), "x must be a dense CUDA tensor"
         for t in (out, residual):
-            assert t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous() and t.device == x.device), \
+            assert t is None or (t.shape == x.shape and t.dtype is x.dtype and t.is_contiguous() and t.get_device() == device), \
                 "out and residual must be dense tensors of x's shape, dtype and device"
-        assert rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous() and rng.device == x.device, \
+        assert rng.dtype is torch.int64 and rng.numel() == 2 and rng.is_contiguous() and rng.get_device() == device, \
             "rng must be int64 (seed, number of the call) on x's device"
+        return device
 
     def dropout_forward(self, out, x, rng, p: float, residual=None) -> None:
         """out = residual + (keep ? x / (1 - p) : 0) (fp32, bf16 or fp16; out may be x or residual).  The mask is drawn
         from rng, an int64 CUDA tensor (seed, number of the call): every call of a model takes a number of its own, and
         dropout_backward the forward pass's pair.  The pair is read on the device, so a replayed CUDA graph that advances
         it draws new masks."""
-        import torch
-        self._dropout_check(out, x, rng, residual)
+        device = self._dropout_check(out, x, rng, residual)
         self._done(self.lib.sideaware_dropout_forward(
             out.data_ptr(), x.data_ptr(), residual.data_ptr() if residual is not None else 0, rng.data_ptr(), p, x.numel(),
-            _dtype_code(x.dtype), x.device.index, _stream_ptr(torch.cuda.current_stream(x.device))), "sideaware_dropout_forward")
+            _dtype_code(x.dtype), device, _current_stream(device)), "sideaware_dropout_forward")
 
     def dropout_backward(self, dx, dout, rng, p: float) -> None:
         """dx = keep ? dout / (1 - p) : 0 with the forward pass's rng (the residual's gradient is dout itself)."""
-        import torch
-        self._dropout_check(dx, dout, rng, None)
+        device = self._dropout_check(dx, dout, rng, None)
         self._done(self.lib.sideaware_dropout_backward(
-            dx.data_ptr(), dout.data_ptr(), rng.data_ptr(), p, dout.numel(), _dtype_code(dout.dtype), dout.device.index,
-            _stream_ptr(torch.cuda.current_stream(dout.device))), "sideaware_dropout_backward")
+            dx.data_ptr(), dout.data_ptr(), rng.data_ptr(), p, dout.numel(), _dtype_code(dout.dtype), device,
+            _current_stream(device)), "sideaware_dropout_backward")
 
     def side_index_tensor(self):
         import torch

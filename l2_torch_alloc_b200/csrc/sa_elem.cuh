@@ -127,6 +127,15 @@ struct Divisor {
 };
 inline Divisor divisor(uint32_t d) { return Divisor{d, d > 1 ? (uint32_t)(0x100000000ull / d + 1) : 0u}; }
 
+// a result that is not read again soon: evict-first
+template <class T, int V>
+__device__ __forceinline__ void sa_store_stream(T* p, const SaVec<T, V>& v) {
+    if constexpr (sizeof(v) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+    else if constexpr (sizeof(v) == 8) __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(&v));
+    else if constexpr (sizeof(v) == 4) __stcs(reinterpret_cast<uint32_t*>(p), *reinterpret_cast<const uint32_t*>(&v));
+    else __stcs(reinterpret_cast<uint16_t*>(p), *reinterpret_cast<const uint16_t*>(&v));
+}
+
 // one entry of a parameter vector (weight, bias) whose type is known at run time only
 __device__ __forceinline__ float sa_param(const void* p, long long i, int dtype) {
     if (dtype == SA_FP32) return static_cast<const float*>(p)[i];

@@ -17,9 +17,13 @@
 //  * for samples too long for that, three launches: partial statistics of runs of rows, joining them, applying them.
 #include <cooperative_groups.h>
 
+#include <mutex>
+#include <set>
 #include <type_traits>
+#include <utility>
 
 #include "sa_elem.cuh"
+#include "sa_kernels.hpp"
 #include "sa_ops.hpp"
 
 namespace cg = cooperative_groups;
@@ -28,39 +32,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kResidentThreads = 512, kResidentBackwardThreads = 256; // threads of a resident block, at most
-constexpr int kBatch = 8; // rows whose statistics a thread takes in one go
 
 struct Norm {
-    long long S, C;         // rows of a sample, channels
-    int G, D;               // groups, channels of a group
-    int splits;             // runs of rows a sample is cut into
-    long long rows;         // rows of a run (the last one may be shorter)
-    int columns, row_lanes; // words across a block's tile, rows it takes at a time
+    long long S, C; // rows of a sample, channels
+    int G, D;       // groups, channels of a group
     int N;
     int silu, param_dtype;
     float eps;
     const void* weight;
     const void* bias;
 };
-
-// V neighbouring entries of a parameter vector, `missing` where there is none.  One branch on the type, then V loads
-// that are in flight together.
-template <int V>
-__device__ __forceinline__ void load_params(float (&out)[V], const void* p, long long c0, int dtype, float missing) {
-    if (!p) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = missing;
-    } else if (dtype == SA_FP32) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = static_cast<const float*>(p)[c0 + i];
-    } else if (dtype == SA_BF16) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c0 + i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = __half2float(static_cast<const __half*>(p)[c0 + i]);
-    }
-}
 
 // mean and sum of squared deviations of `n` values
 struct Moments {
@@ -83,296 +64,16 @@ __device__ __forceinline__ float sigmoid(float z) {
     return __fdividef(1.0f, 1.0f + __expf(-z));
 }
 
-template <class T>
-__device__ __forceinline__ float activate(float z, int silu) {
-    return silu ? z * sigmoid<T>(z) : z;
-}
-
-// dy act'(z)
-template <class T>
-__device__ __forceinline__ float through_activation(float dy, float z, int silu) {
-    if (!silu) return dy;
-    const float s = sigmoid<T>(z);
-    return dy * (s * fmaf(z, 1.0f - s, 1.0f));
-}
-
 // ---------------------------------------------------------------------------
-// forward
-// ---------------------------------------------------------------------------
-// partial[n][split][c] = (mean, m2) of channel c over the run's rows
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads)
-sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, const __grid_constant__ Norm p) {
-    __shared__ float2 tile[kThreads * V];
-    __shared__ float count[kThreads];
-    const int lane_column = threadIdx.x % p.columns, row_lane = threadIdx.x / p.columns;
-    const long long c0 = ((long long)blockIdx.y * p.columns + lane_column) * V;
-    const int split = blockIdx.x % p.splits, n = blockIdx.x / p.splits;
-    const long long first = split * p.rows, end = min(first + p.rows, p.S);
-    const bool mine = row_lane < p.row_lanes && c0 < p.C;
-    Moments a[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = Moments{0.0f, 0.0f, 0.0f};
-    if (mine) {
-        const T* base = x + ((long long)n * p.S) * p.C + c0;
-        for (long long s = first + row_lane; s < end; s += (long long)kBatch * p.row_lanes) {
-            SaVec<T, V> v[kBatch];
-            int have = 0;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k)
-                if (s + (long long)k * p.row_lanes < end) {
-                    v[k] = sa_load<T, V>(base + (s + (long long)k * p.row_lanes) * p.C);
-                    have = k + 1;
-                }
-            const float inv = 1.0f / (float)have;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float sum = 0.0f, m2 = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) sum += k < have ? sa_to_float(v[k].e[i]) : 0.0f;
-                const float mean = sum * inv;
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const float d = k < have ? sa_to_float(v[k].e[i]) - mean : 0.0f;
-                    m2 = fmaf(d, d, m2);
-                }
-                join(a[i], Moments{(float)have, mean, m2});
-            }
-        }
-    }
-    count[threadIdx.x] = mine ? a[0].n : 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) tile[threadIdx.x * V + i] = make_float2(a[i].mean, a[i].m2);
-    __syncthreads();
-    // the tile's channels, each over its row lanes
-    for (int j = threadIdx.x; j < p.columns * V; j += kThreads) {
-        const long long c = (long long)blockIdx.y * p.columns * V + j;
-        if (c >= p.C) continue;
-        Moments m{0.0f, 0.0f, 0.0f};
-        for (int r = 0; r < p.row_lanes; ++r) {
-            const int t = r * p.columns + j / V;
-            const float2 e = tile[t * V + j % V];
-            join(m, Moments{count[t], e.x, e.y});
-        }
-        partial[((long long)n * p.splits + split) * p.C + c] = make_float2(m.mean, m.m2);
-    }
-}
-
-__device__ __forceinline__ Moments warp_join(Moments m) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Moments b{__shfl_down_sync(0xffffffffu, m.n, o), __shfl_down_sync(0xffffffffu, m.mean, o), __shfl_down_sync(0xffffffffu, m.m2, o)};
-        join(m, b);
-    }
-    return m;
-}
-
-// mean and rstd of (n, g): one block each
-__global__ void __launch_bounds__(kThreads)
-sa_norm_join_kernel(const float2* __restrict__ partial, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Norm p) {
-    __shared__ Moments warps[kThreads / 32];
-    const int n = blockIdx.x / p.G, g = blockIdx.x % p.G;
-    Moments m{0.0f, 0.0f, 0.0f};
-    const long long entries = (long long)p.splits * p.D;
-    for (long long i = threadIdx.x; i < entries; i += kThreads) {
-        const long long split = i / p.D;
-        const long long rows = min(p.rows, p.S - split * p.rows);
-        const float2 e = partial[((long long)n * p.splits + split) * p.C + (long long)g * p.D + i % p.D];
-        join(m, Moments{(float)rows, e.x, e.y});
-    }
-    m = warp_join(m);
-    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = m;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        m = threadIdx.x < kThreads / 32 ? warps[threadIdx.x] : Moments{0.0f, 0.0f, 0.0f};
-        m = warp_join(m);
-        if (threadIdx.x == 0) {
-            mean[blockIdx.x] = m.mean;
-            rstd[blockIdx.x] = 1.0f / sqrtf(m.m2 / m.n + p.eps);
-        }
-    }
-}
-
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads)
-sa_norm_apply_kernel(T* out, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd, const __grid_constant__ Norm p) {
-    const int lane_column = threadIdx.x % p.columns, row_lane = threadIdx.x / p.columns;
-    const long long c0 = ((long long)blockIdx.y * p.columns + lane_column) * V;
-    if (row_lane >= p.row_lanes || c0 >= p.C) return;
-    const int split = blockIdx.x % p.splits, n = blockIdx.x / p.splits;
-    float m[V], a[V], b[V];
-    load_params<V>(a, p.weight, c0, p.param_dtype, 1.0f);
-    load_params<V>(b, p.bias, c0, p.param_dtype, 0.0f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const long long at = (long long)n * p.G + (uint32_t)(c0 + i) / (uint32_t)p.D;
-        m[i] = mean[at];
-        a[i] *= rstd[at];
-    }
-    const long long first = split * p.rows, end = min(first + p.rows, p.S);
-    const long long base = (long long)n * p.S * p.C + c0;
-#pragma unroll 4
-    for (long long s = first + row_lane; s < end; s += p.row_lanes) {
-        SaVec<T, V> v = sa_load_stream<T, V>(x + base + s * p.C);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            v.e[i] = sa_from_float<T>(activate<T>(fmaf(sa_to_float(v.e[i]) - m[i], a[i], b[i]), p.silu));
-        sa_store<T, V>(out + base + s * p.C, v);
-    }
-}
-
-// ---------------------------------------------------------------------------
-// backward
-// ---------------------------------------------------------------------------
-// partial[n][split][c] = (sum dz, sum dz u) over the run's rows
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict__ x, const float* __restrict__ mean,
-                                const float* __restrict__ rstd, float2* __restrict__ partial, const __grid_constant__ Norm p) {
-    __shared__ float2 tile[kThreads * V];
-    const int lane_column = threadIdx.x % p.columns, row_lane = threadIdx.x / p.columns;
-    const long long c0 = ((long long)blockIdx.y * p.columns + lane_column) * V;
-    const int split = blockIdx.x % p.splits, n = blockIdx.x / p.splits;
-    const long long first = split * p.rows, end = min(first + p.rows, p.S);
-    const bool mine = row_lane < p.row_lanes && c0 < p.C;
-    float sa[V], sb[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.0f;
-    if (mine) {
-        float m[V], r[V], w[V], b[V];
-        load_params<V>(w, p.weight, c0, p.param_dtype, 1.0f);
-        load_params<V>(b, p.bias, c0, p.param_dtype, 0.0f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const long long at = (long long)n * p.G + (uint32_t)(c0 + i) / (uint32_t)p.D;
-            m[i] = mean[at];
-            r[i] = rstd[at];
-        }
-        const long long base = (long long)n * p.S * p.C + c0;
-#pragma unroll 4
-        for (long long s = first + row_lane; s < end; s += p.row_lanes) {
-            const SaVec<T, V> vx = sa_load<T, V>(x + base + s * p.C), vd = sa_load<T, V>(dout + base + s * p.C);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float u = (sa_to_float(vx.e[i]) - m[i]) * r[i];
-                const float dz = through_activation<T>(sa_to_float(vd.e[i]), fmaf(u, w[i], b[i]), p.silu);
-                sa[i] += dz;
-                sb[i] = fmaf(dz, u, sb[i]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) tile[threadIdx.x * V + i] = make_float2(sa[i], sb[i]);
-    __syncthreads();
-    for (int j = threadIdx.x; j < p.columns * V; j += kThreads) {
-        const long long c = (long long)blockIdx.y * p.columns * V + j;
-        if (c >= p.C) continue;
-        float2 sum = make_float2(0.0f, 0.0f);
-        for (int q = 0; q < p.row_lanes; ++q) {
-            const float2 e = tile[(q * p.columns + j / V) * V + j % V];
-            sum.x += e.x;
-            sum.y += e.y;
-        }
-        partial[((long long)n * p.splits + split) * p.C + c] = sum;
-    }
-}
-
-// sums[n][c] over the runs, and of every (n, g) m1 and m2: one block each
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_join_kernel(const float2* __restrict__ partial, float2* __restrict__ sums, float2* __restrict__ means,
-                             const __grid_constant__ Norm p) {
-    __shared__ float2 warps[kThreads / 32];
-    const int n = blockIdx.x / p.G, g = blockIdx.x % p.G;
-    float2 m = make_float2(0.0f, 0.0f);
-    for (int d = threadIdx.x; d < p.D; d += kThreads) {
-        const long long c = (long long)g * p.D + d;
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int k = 0; k < p.splits; ++k) {
-            const float2 e = partial[((long long)n * p.splits + k) * p.C + c];
-            s.x += e.x;
-            s.y += e.y;
-        }
-        sums[(long long)n * p.C + c] = s;
-        const float w = p.weight ? sa_param(p.weight, c, p.param_dtype) : 1.0f;
-        m.x = fmaf(w, s.x, m.x);
-        m.y = fmaf(w, s.y, m.y);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        m.x += __shfl_down_sync(0xffffffffu, m.x, o);
-        m.y += __shfl_down_sync(0xffffffffu, m.y, o);
-    }
-    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < kThreads / 32; ++k) {
-            m.x += warps[k].x;
-            m.y += warps[k].y;
-        }
-        const float inv = 1.0f / ((float)p.S * (float)p.D);
-        means[blockIdx.x] = make_float2(m.x * inv, m.y * inv);
-    }
-}
-
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict__ dweight, void* __restrict__ dbias, const __grid_constant__ Norm p) {
-    const long long c = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (c >= p.C) return;
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int n = 0; n < p.N; ++n) {
-        const float2 e = sums[(long long)n * p.C + c];
-        s.x += e.x;
-        s.y += e.y;
-    }
-    if (dbias) sa_set_param(dbias, c, p.param_dtype, s.x);
-    if (dweight) sa_set_param(dweight, c, p.param_dtype, s.y);
-}
-
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
-                              const float2* __restrict__ means, const __grid_constant__ Norm p) {
-    const int lane_column = threadIdx.x % p.columns, row_lane = threadIdx.x / p.columns;
-    const long long c0 = ((long long)blockIdx.y * p.columns + lane_column) * V;
-    if (row_lane >= p.row_lanes || c0 >= p.C) return;
-    const int split = blockIdx.x % p.splits, n = blockIdx.x / p.splits;
-    float m[V], r[V], w[V], b[V], m1[V], m2[V];
-    load_params<V>(w, p.weight, c0, p.param_dtype, 1.0f);
-    load_params<V>(b, p.bias, c0, p.param_dtype, 0.0f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const long long at = (long long)n * p.G + (uint32_t)(c0 + i) / (uint32_t)p.D;
-        m[i] = mean[at];
-        r[i] = rstd[at];
-        m1[i] = means[at].x;
-        m2[i] = means[at].y;
-    }
-    const long long first = split * p.rows, end = min(first + p.rows, p.S);
-    const long long base = (long long)n * p.S * p.C + c0;
-#pragma unroll 2
-    for (long long s = first + row_lane; s < end; s += p.row_lanes) {
-        const SaVec<T, V> vx = sa_load_stream<T, V>(x + base + s * p.C), vd = sa_load_stream<T, V>(dout + base + s * p.C);
-        SaVec<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float u = (sa_to_float(vx.e[i]) - m[i]) * r[i];
-            const float dz = through_activation<T>(sa_to_float(vd.e[i]), fmaf(u, w[i], b[i]), p.silu);
-            o.e[i] = sa_from_float<T>(r[i] * (fmaf(w[i], dz, -m1[i]) - u * m2[i]));
-        }
-        sa_store<T, V>(dx + base + s * p.C, o);
-    }
-}
-
-// ---------------------------------------------------------------------------
-// resident: a cluster for a slab of groups of one sample
+// what the kernels share: a block has some rows of a slab (neighbouring channels) of one sample
 // ---------------------------------------------------------------------------
 struct Slab {
     Norm p;
-    int groups, width;     // groups of a slab, its channels = groups * D, a whole number of words
+    int groups, width;     // channels of a slab, a whole number of words; resident: whole groups, so many
     int words;             // words of a row
     int row_lanes;         // rows a block takes at a time: a thread has one word of every row_lanes-th row
     int slabs;             // of a sample
-    int blocks;            // of a cluster
+    int blocks;            // of a slab of a sample; resident: a cluster
     int rows;              // of a block
     int parts;             // threads that share a channel's column when the block's threads are joined
     int threads;
@@ -392,10 +93,10 @@ struct Place {
 };
 
 template <int V>
-__device__ __forceinline__ Place place_of(const Slab& s) {
+__device__ __forceinline__ Place place_of(const Slab& s, uint32_t block) {
     Place w;
-    const uint32_t cluster = s.blocks > 1 ? blockIdx.x / (uint32_t)s.blocks : blockIdx.x;
-    w.rank = (int)(blockIdx.x - cluster * s.blocks);
+    const uint32_t cluster = s.blocks > 1 ? block / (uint32_t)s.blocks : block;
+    w.rank = (int)(block - cluster * s.blocks);
     w.n = (int)(cluster / (uint32_t)s.slabs);
     const int slab = (int)cluster - w.n * s.slabs;
     w.row_lane = (int)s.by_words.div(threadIdx.x);
@@ -403,8 +104,8 @@ __device__ __forceinline__ Place place_of(const Slab& s) {
     w.group0 = slab * s.groups;
     w.first = (long long)slab * s.width;
     w.groups = min(s.groups, s.p.G - w.group0);
-    w.channels = w.groups * s.p.D;
-    w.block_rows = max(0, min(s.rows, (int)s.p.S - w.rank * s.rows)); // a sample that fits is short
+    w.channels = (int)min((long long)s.width, s.p.C - w.first);
+    w.block_rows = (int)max(0ll, min((long long)s.rows, s.p.S - (long long)w.rank * s.rows));
     const int left = w.block_rows - w.row_lane;
     w.rows = w.row_lane < s.row_lanes && w.word * V < w.channels && left > 0 ? (left + s.row_lanes - 1) / s.row_lanes : 0;
     return w;
@@ -417,16 +118,18 @@ constexpr int kStages = 4;
 __device__ __forceinline__ int stage_end(int rows, int stage) { return stage == kStages - 1 ? rows : rows * (stage + 1) / kStages; }
 
 template <class T, int V>
+__device__ __forceinline__ void fetch_row(SaVec<T, V>* to, const T* from) {
+    if constexpr (sizeof(SaVec<T, V>) == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+    else if constexpr (sizeof(SaVec<T, V>) >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(sizeof(SaVec<T, V>)) : "memory");
+    else
+        *to = sa_load<T, V>(from);
+}
+template <class T, int V>
 __device__ __forceinline__ void fetch_rows(SaVec<T, V>* to, const T* from, int rows, int stride, long long step) {
 #pragma unroll 4
-    for (int u = 0; u < rows; ++u, to += stride, from += step) {
-        if constexpr (sizeof(SaVec<T, V>) == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-        else if constexpr (sizeof(SaVec<T, V>) >= 4)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(sizeof(SaVec<T, V>)) : "memory");
-        else
-            *to = sa_load<T, V>(from);
-    }
+    for (int u = 0; u < rows; ++u, to += stride, from += step) fetch_row<T, V>(to, from);
 }
 __device__ __forceinline__ void end_of_stage() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int STAGE>
@@ -497,6 +200,15 @@ __device__ __forceinline__ void column_sums(const Slab& s, int lanes, float2* ti
     }
 }
 
+__device__ __forceinline__ Moments warp_join(Moments m) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Moments b{__shfl_down_sync(0xffffffffu, m.n, o), __shfl_down_sync(0xffffffffu, m.mean, o), __shfl_down_sync(0xffffffffu, m.m2, o)};
+        join(m, b);
+    }
+    return m;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -557,6 +269,454 @@ __device__ __forceinline__ void block_sums(const Slab& s, const Place& w, float2
     __syncthreads();
 }
 
+// Row lane 0's means for everybody; a barrier has to follow.
+template <int V>
+__device__ __forceinline__ void share_centre(const Place& w, const F2 (&m)[(V + 1) / 2], float* centre) {
+    if (w.row_lane == 0) {
+#pragma unroll
+        for (int k = 0; k < (V + 1) / 2; ++k) {
+            float mx, my;
+            split(m[k], mx, my);
+            centre[w.word * V + 2 * k] = mx;
+            if (2 * k + 1 < V) centre[w.word * V + 2 * k + 1] = my;
+        }
+    }
+}
+
+// (mean, m2) of this thread's n rows become the sums of x - centre and of its square.
+template <int V>
+__device__ __forceinline__ void refer_to_centre(const Place& w, F2 (&m)[(V + 1) / 2], F2 (&q)[(V + 1) / 2], float n, const float* centre) {
+    if (w.rows <= 0) return; // without rows both are 0
+    F2 c[(V + 1) / 2];
+    shared_pairs<V>(c, centre + w.word * V);
+#pragma unroll
+    for (int k = 0; k < (V + 1) / 2; ++k) {
+        const F2 d = m[k] + negative(c[k]);
+        m[k] = f2(n, n) * d;
+        q[k] = fma2(m[k], d, q[k]);
+    }
+}
+
+// channel c's sums once block_sums is through
+template <int V>
+__device__ __forceinline__ float2 channel_sum(const Slab& s, const float2* tile, int c) {
+    const float2* const at = tile + tile_place<V>(s, c);
+    float2 t = *at;
+    for (int part = 1; part < s.parts; ++part) {
+        const float2 e = at[part * s.width];
+        t.x += e.x;
+        t.y += e.y;
+    }
+    return t;
+}
+
+// ---------------------------------------------------------------------------
+// samples too long for that: partial results of runs of rows, joined, then applied
+// ---------------------------------------------------------------------------
+// A thread's rows (one word of each) on their way through a ring in shared memory that only this thread uses: four stages of
+// ROWS rows are in flight.  16 words of each thread in all (64 KiB of a block, three blocks of an SM): 4 rows of one tensor or
+// 2 of two.
+constexpr int kStreamStages = 4, kRingWords = 16;
+
+template <class T, int V>
+struct Stream {
+    SaVec<T, V>* ring; // [rows][kThreads], this thread's column
+    const T* from;
+    long long step;
+    __device__ __forceinline__ Stream(void* memory, const T* first, long long rows_apart)
+        : ring((SaVec<T, V>*)memory + threadIdx.x), from(first), step(rows_apart) {}
+    __device__ __forceinline__ void fetch(int slot) {
+        fetch_row<T, V>(ring + slot * kThreads, from);
+        from += step;
+    }
+    __device__ __forceinline__ SaVec<T, V> row(int slot) const { return ring[slot * kThreads]; }
+};
+
+// fetch(slot) sets the next row under way, f(slot) works on the row in a slot; stage(slot, rows) comes before a stage's rows.
+// Slots are constants once the loops are unrolled, and a whole stage takes one test.
+template <int ROWS, class Fetch, class Stage, class F>
+__device__ __forceinline__ void stream_rows(int rows, Fetch&& fetch, Stage&& stage, F&& f) {
+    auto fetch_stage = [&](int slot, int left) {
+        if (left >= ROWS) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) fetch(slot + r);
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (r < left) fetch(slot + r);
+        }
+        end_of_stage();
+    };
+    int left = rows, ahead = rows; // rows to work on, rows to fetch
+#pragma unroll
+    for (int k = 0; k < kStreamStages; ++k, ahead -= ROWS) fetch_stage(k * ROWS, ahead);
+    while (left > 0) {
+#pragma unroll
+        for (int k = 0; k < kStreamStages; ++k) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStreamStages - 1) : "memory");
+            if (left >= ROWS) {
+                stage(k * ROWS, ROWS);
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) f(k * ROWS + r);
+            } else if (left > 0) {
+                stage(k * ROWS, left);
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r)
+                    if (r < left) f(k * ROWS + r);
+            }
+            fetch_stage(k * ROWS, ahead);
+            left -= ROWS;
+            ahead -= ROWS;
+        }
+    }
+}
+
+// Kernels of one call overlap their launches (programmatic dependent launch): a later one waits here before it reads
+// what an earlier one wrote.
+__device__ __forceinline__ void may_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// partial[n][run][c] = (mean, m2) of channel c over the run's rows
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 3)
+sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    float2* const tile = (float2*)memory;                                   // [lanes][width], after the stream has passed
+    float* const centre = (float*)(memory + s.shared); // [width] the means of row lane 0
+    may_follow();
+    const Place w = place_of<V>(s, blockIdx.x);
+    const Norm& p = s.p;
+    // sums about the first of every kFold rows (what cancels is of the size of a value's own square), joined by Chan's rule
+    constexpr int kFold = 32, kRows = kRingWords / kStreamStages;
+    F2 k0[P], sum[P], square[P], m[P], q[P];
+    float n = 0.0f;
+    int have = 0;
+#pragma unroll
+    for (int k = 0; k < P; ++k) k0[k] = sum[k] = square[k] = m[k] = q[k] = f2(0.0f, 0.0f);
+    auto fold = [&] {
+        const float c = (float)have, inv = 1.0f / c, share = __fdividef(c, n + c), weight = n * share;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            const F2 part = sum[k] * f2(inv, inv), d = part + negative(k0[k] + m[k]);
+            q[k] = q[k] + fma2(negative(sum[k]), part, square[k]);
+            q[k] = fma2(d * d, f2(weight, weight), q[k]);
+            m[k] = fma2(d, f2(share, share), m[k]);
+            sum[k] = square[k] = f2(0.0f, 0.0f);
+        }
+        n += c;
+        have = 0;
+    };
+    Stream<T, V> in(memory, x + ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V,
+                    (long long)s.row_lanes * p.C);
+    stream_rows<kRows>(
+        w.rows, [&](int slot) { in.fetch(slot); },
+        [&](int slot, int rows) {
+            if (have == kFold) fold();
+            if (have == 0) {
+                const SaVec<T, V> v = in.row(slot);
+#pragma unroll
+                for (int k = 0; k < P; ++k) k0[k] = negative(pair_of(v, k));
+            }
+            have += rows;
+        },
+        [&](int slot) {
+            const SaVec<T, V> v = in.row(slot);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const F2 e = pair_of(v, k) + k0[k];
+                sum[k] = sum[k] + e;
+                square[k] = fma2(e, e, square[k]);
+            }
+        });
+    if (have > 0) fold();
+    __syncthreads(); // the ring becomes the tile
+    share_centre<V>(w, m, centre);
+    __syncthreads();
+    refer_to_centre<V>(w, m, q, n, centre);
+    block_sums<V>(s, w, tile, m, q);
+    const float rows_inv = w.block_rows > 0 ? 1.0f / (float)w.block_rows : 0.0f;
+    for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
+        const float2 t = channel_sum<V>(s, tile, j);
+        const float off = t.x * rows_inv;
+        partial[((long long)w.n * s.blocks + w.rank) * p.C + w.first + j] = make_float2(centre[j] + off, fmaf(-t.x, off, t.y));
+    }
+}
+
+// mean and rstd of (n, g): one block each
+__global__ void __launch_bounds__(kThreads)
+sa_norm_join_kernel(const float2* __restrict__ partial, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Slab s) {
+    __shared__ Moments warps[kThreads / 32];
+    may_follow();
+    const Norm& p = s.p;
+    const uint32_t n = blockIdx.x / (uint32_t)p.G, g = blockIdx.x - n * (uint32_t)p.G;
+    // some threads for each channel, each a share of the runs; channels beyond the block's width in turn
+    const int wide = min(p.D, kThreads), shares = kThreads / wide;
+    const int share = threadIdx.x / wide, lane = threadIdx.x - share * wide;
+    const float last = (float)(p.S - (long long)(s.blocks - 1) * s.rows);
+    Moments m{0.0f, 0.0f, 0.0f};
+    await_previous();
+    if (share < shares) {
+        for (int d = lane; d < p.D; d += wide) {
+            const float2* const from = partial + (long long)n * s.blocks * p.C + (long long)g * p.D + d;
+#pragma unroll 8
+            for (int r = share; r < s.blocks; r += shares) {
+                const float2 e = from[(long long)r * p.C];
+                join(m, Moments{r + 1 == s.blocks ? last : (float)s.rows, e.x, e.y});
+            }
+        }
+    }
+    m = warp_join(m);
+    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = m;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = threadIdx.x < kThreads / 32 ? warps[threadIdx.x] : Moments{0.0f, 0.0f, 0.0f};
+        m = warp_join(m);
+        if (threadIdx.x == 0) {
+            mean[blockIdx.x] = m.mean;
+            rstd[blockIdx.x] = 1.0f / sqrtf(m.m2 / m.n + p.eps);
+        }
+    }
+}
+
+// The rows are taken from the end: what the statistics read last is still in L2.
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 3)
+sa_norm_apply_kernel(T* out, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    float* const weight = (float*)(memory + s.shared); // [width] each: weight * rstd, bias, mean
+    float* const bias = weight + s.width;
+    float* const centre = bias + s.width;
+    const Place w = place_of<V>(s, gridDim.x - 1 - blockIdx.x);
+    const Norm& p = s.p;
+    stage_params(s, w, weight, bias);
+    await_previous();
+    for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
+        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        centre[j] = mean[at];
+        weight[j] *= rstd[at];
+    }
+    __syncthreads();
+    if (w.rows <= 0) return;
+    F2 m[P], a[P], b[P];
+    shared_pairs<V>(m, centre + w.word * V);
+    shared_pairs<V>(a, weight + w.word * V);
+    shared_pairs<V>(b, bias + w.word * V);
+#pragma unroll
+    for (int k = 0; k < P; ++k) m[k] = negative(m[k]);
+    const long long step = (long long)s.row_lanes * p.C;
+    const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V + (w.rows - 1) * step;
+    Stream<T, V> in(memory, x + base, -step);
+    T* to = out + base;
+    stream_rows<kRingWords / kStreamStages>(
+        w.rows, [&](int slot) { in.fetch(slot); }, [](int, int) {},
+        [&](int slot) {
+            SaVec<T, V> v = in.row(slot);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const F2 z = fma2(pair_of(v, k) + m[k], a[k], b[k]);
+                set_pair(v, k, p.silu ? z * sigmoid2<T>(z) : z);
+            }
+            sa_store_stream<T, V>(to, v);
+            to -= step;
+        });
+}
+
+// partial[n][run][c] = (sum dz, sum dz (x - mean)) over the run's rows
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 3)
+sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict__ x, const float* __restrict__ mean,
+                                const float* __restrict__ rstd, float2* __restrict__ partial, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    constexpr int kRows = kRingWords / 2 / kStreamStages;
+    constexpr size_t kRing = kRingWords / 2 * kThreads * sizeof(SaVec<T, V>);
+    float2* const tile = (float2*)memory;              // [lanes][width], after the streams have passed
+    float* const slope = (float*)(memory + s.shared); // [width] each: weight * rstd, bias, mean
+    float* const bias = slope + s.width;
+    float* const centre = bias + s.width;
+    may_follow();
+    const Place w = place_of<V>(s, blockIdx.x);
+    const Norm& p = s.p;
+    stage_params(s, w, slope, bias);
+    for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
+        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        centre[j] = mean[at];
+        slope[j] *= rstd[at];
+    }
+    __syncthreads();
+    F2 m[P], sl[P], b[P], a0[P], a1[P];
+    if (w.row_lane < s.row_lanes) {
+        shared_pairs<V>(m, centre + w.word * V);
+        shared_pairs<V>(sl, slope + w.word * V);
+        shared_pairs<V>(b, bias + w.word * V);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        m[k] = negative(m[k]);
+        a0[k] = a1[k] = f2(0.0f, 0.0f);
+    }
+    const long long step = (long long)s.row_lanes * p.C;
+    const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V;
+    Stream<T, V> in(memory, x + base, step), grad(memory + kRing, dout + base, step);
+    stream_rows<kRows>(
+        w.rows,
+        [&](int slot) {
+            in.fetch(slot);
+            grad.fetch(slot);
+        },
+        [](int, int) {},
+        [&](int slot) {
+            const SaVec<T, V> v = in.row(slot), d = grad.row(slot);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const F2 dev = pair_of(v, k) + m[k];
+                const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
+                a0[k] = a0[k] + dz;
+                a1[k] = fma2(dz, dev, a1[k]);
+            }
+        });
+    __syncthreads(); // the rings become the tile
+    block_sums<V>(s, w, tile, a0, a1);
+    for (int j = threadIdx.x; j < w.channels; j += blockDim.x)
+        partial[((long long)w.n * s.blocks + w.rank) * p.C + w.first + j] = channel_sum<V>(s, tile, j);
+}
+
+// sums[n][c] = (sum dz, sum dz u), and of every (n, g) (-rstd m1, -rstd^2 m2): one block for each (n, g)
+__global__ void __launch_bounds__(kThreads)
+sa_norm_backward_join_kernel(const float2* __restrict__ partial, const float* __restrict__ rstd, float2* __restrict__ sums,
+                             float2* __restrict__ means, const __grid_constant__ Slab s) {
+    __shared__ float2 tile[kThreads];
+    may_follow();
+    await_previous();
+    const Norm& p = s.p;
+    const uint32_t n = blockIdx.x / (uint32_t)p.G, g = blockIdx.x - n * (uint32_t)p.G;
+    const float rs = rstd[blockIdx.x];
+    // some threads for each channel, each a share of the runs; channels beyond the block's width in turn
+    const int wide = min(p.D, kThreads), shares = kThreads / wide;
+    const int share = threadIdx.x / wide, lane = threadIdx.x - share * wide;
+    float2 m = make_float2(0.0f, 0.0f);
+    for (int d0 = 0; d0 < p.D; d0 += wide) {
+        const long long c = (long long)g * p.D + d0 + lane;
+        const bool mine = d0 + lane < p.D && share < shares;
+        float2 t = make_float2(0.0f, 0.0f);
+        if (mine) {
+#pragma unroll 4
+            for (int r = share; r < s.blocks; r += shares) {
+                const float2 e = partial[((long long)n * s.blocks + r) * p.C + c];
+                t.x += e.x;
+                t.y += e.y;
+            }
+        }
+        tile[threadIdx.x] = t;
+        __syncthreads();
+        if (mine && share == 0) {
+            for (int q = 1; q < shares; ++q) {
+                t.x += tile[q * wide + lane].x;
+                t.y += tile[q * wide + lane].y;
+            }
+            t.y *= rs;
+            sums[(long long)n * p.C + c] = t;
+            const float w = p.weight ? sa_param(p.weight, c, p.param_dtype) : 1.0f;
+            m.x = fmaf(w, t.x, m.x);
+            m.y = fmaf(w, t.y, m.y);
+        }
+        __syncthreads();
+    }
+    m = make_float2(warp_sum(m.x), warp_sum(m.y));
+    if (threadIdx.x % 32 == 0) tile[threadIdx.x / 32] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < kThreads / 32; ++k) {
+            m.x += tile[k].x;
+            m.y += tile[k].y;
+        }
+        const float inv = 1.0f / ((float)p.S * (float)p.D);
+        means[blockIdx.x] = make_float2(-rs * (m.x * inv), -rs * (m.y * inv) * rs);
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict__ dweight, void* __restrict__ dbias, const __grid_constant__ Norm p) {
+    await_previous();
+    const long long c = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (c >= p.C) return;
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int n = 0; n < p.N; ++n) {
+        const float2 e = sums[(long long)n * p.C + c];
+        s.x += e.x;
+        s.y += e.y;
+    }
+    if (dbias) sa_set_param(dbias, c, p.param_dtype, s.x);
+    if (dweight) sa_set_param(dweight, c, p.param_dtype, s.y);
+}
+
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 3)
+sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
+                              const float2* __restrict__ means, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    constexpr int kRows = kRingWords / 2 / kStreamStages;
+    constexpr size_t kRing = kRingWords / 2 * kThreads * sizeof(SaVec<T, V>);
+    float* const slope = (float*)(memory + s.shared); // [width] each: weight * rstd, bias, mean, the two means of the gradient
+    float* const bias = slope + s.width;
+    float* const centre = bias + s.width;
+    float* const first = centre + s.width;
+    float* const second = first + s.width;
+    const Place w = place_of<V>(s, gridDim.x - 1 - blockIdx.x);
+    const Norm& p = s.p;
+    may_follow();
+    stage_params(s, w, slope, bias);
+    await_previous();
+    for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
+        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        centre[j] = mean[at];
+        slope[j] *= rstd[at];
+        const float2 e = means[at];
+        first[j] = e.x;
+        second[j] = e.y;
+    }
+    __syncthreads();
+    if (w.rows <= 0) return;
+    F2 m[P], sl[P], b[P], m1[P], m2[P];
+    shared_pairs<V>(m, centre + w.word * V);
+    shared_pairs<V>(sl, slope + w.word * V);
+    shared_pairs<V>(b, bias + w.word * V);
+    shared_pairs<V>(m1, first + w.word * V);
+    shared_pairs<V>(m2, second + w.word * V);
+#pragma unroll
+    for (int k = 0; k < P; ++k) m[k] = negative(m[k]);
+    const long long step = (long long)s.row_lanes * p.C;
+    const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V + (w.rows - 1) * step;
+    Stream<T, V> in(memory, x + base, -step), grad(memory + kRing, dout + base, -step);
+    T* to = dx + base;
+    stream_rows<kRows>(
+        w.rows,
+        [&](int slot) {
+            in.fetch(slot);
+            grad.fetch(slot);
+        },
+        [](int, int) {},
+        [&](int slot) {
+            SaVec<T, V> v = in.row(slot);
+            const SaVec<T, V> d = grad.row(slot);
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const F2 dev = pair_of(v, k) + m[k];
+                const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
+                set_pair(v, k, fma2(dev, m2[k], fma2(sl[k], dz, m1[k])));
+            }
+            sa_store_stream<T, V>(to, v);
+            to -= step;
+        });
+}
+
+// ---------------------------------------------------------------------------
+// resident: a cluster for a slab of groups of one sample
+// ---------------------------------------------------------------------------
 // Statistics of a thread: sums of x - K and of its square, K being the thread's first row.  What cancels when they are put
 // together is of the size of K's own square, and K is one of a few values: nothing is lost.  The block's threads then refer
 // their sums to the mean of row lane 0 (the same argument, with its rows among the block's), which makes them plain sums;
@@ -572,7 +732,7 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
     float* const weight = (float*)(joined + s.groups); // [width] each: weight, then weight * rstd; bias; the means of row lane 0, then the groups'
     float* const bias = weight + s.width;
     float* const centre = bias + s.width;
-    const Place w = place_of<V>(s);
+    const Place w = place_of<V>(s, blockIdx.x);
     const Norm& p = s.p;
 
     const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V;
@@ -618,26 +778,9 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
             m[k] = part + negative(k0[k]);
         }
     }
-    if (w.row_lane == 0) {
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-            float mx, my;
-            split(m[k], mx, my);
-            centre[w.word * V + 2 * k] = mx;
-            if (2 * k + 1 < V) centre[w.word * V + 2 * k + 1] = my;
-        }
-    }
+    share_centre<V>(w, m, centre);
     __syncthreads();
-    if (w.rows > 0) { // without rows both stay 0
-        F2 c[P];
-        shared_pairs<V>(c, centre + w.word * V);
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-            const F2 d = m[k] + negative(c[k]);
-            m[k] = f2(n, n) * d;
-            q[k] = fma2(m[k], d, q[k]);
-        }
-    }
+    refer_to_centre<V>(w, m, q, n, centre);
     block_sums<V>(s, w, tile, m, q);
     // a warp for each group
     const float rows_inv = w.block_rows > 0 ? 1.0f / (float)w.block_rows : 0.0f, D_inv = 1.0f / (float)p.D;
@@ -645,15 +788,9 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
         float sum = 0.0f, m2 = 0.0f;
         for (int d = threadIdx.x % 32; d < p.D; d += 32) { // a channel's mean and squared deviations
             const int c = g * p.D + d;
-            float2* const at = tile + tile_place<V>(s, c);
-            float2 t = *at;
-            for (int part = 1; part < s.parts; ++part) {
-                const float2 e = at[part * s.width];
-                t.x += e.x;
-                t.y += e.y;
-            }
+            const float2 t = channel_sum<V>(s, tile, c);
             const float off = t.x * rows_inv, mc = centre[c] + off;
-            at->x = mc;
+            tile[tile_place<V>(s, c)].x = mc;
             m2 += fmaf(-t.x, off, t.y);
             sum += mc;
         }
@@ -736,7 +873,7 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
     float* const bias = weight + s.width;
     float* const centre = bias + s.width;
     float* const slope = centre + s.width; // weight * rstd
-    const Place w = place_of<V>(s);
+    const Place w = place_of<V>(s, blockIdx.x);
     const Norm& p = s.p;
 
     const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V;
@@ -787,16 +924,7 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
         });
         block_sums<V>(s, w, tile, a0, a1);
     }
-    for (int j = threadIdx.x; j < s.width; j += blockDim.x) {
-        const float2* const at = tile + tile_place<V>(s, j);
-        float2 t = *at;
-        for (int part = 1; part < s.parts; ++part) {
-            const float2 e = at[part * s.width];
-            t.x += e.x;
-            t.y += e.y;
-        }
-        channel[j] = t;
-    }
+    for (int j = threadIdx.x; j < s.width; j += blockDim.x) channel[j] = channel_sum<V>(s, tile, j);
     cg::cluster_group cluster = cg::this_cluster();
     if (s.blocks > 1) cluster.sync();
     else __syncthreads();
@@ -870,19 +998,31 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// How a sample is cut: words across a block, rows at a time, runs of rows.  About four blocks for each SM, but runs of
-// at least `kBatch` rows for each row lane, so that partial results stay a small part of the traffic.
-void cut(Norm& p, int V, int* column_tiles) {
+// Samples too long to be resident: words across a block, rows at a time, runs of rows.  Three blocks for each SM, but runs
+// of at least 32 rows for each row lane, so that partial results stay a small part of the traffic.
+Slab cut(const Norm& p, int V) {
+    Slab s{};
+    s.p = p;
     const long long words = p.C / V;
-    p.columns = (int)(words < kThreads ? words : kThreads);
-    p.row_lanes = kThreads / p.columns;
-    *column_tiles = (int)((words + p.columns - 1) / p.columns);
-    long long splits = 148 * 4 / ((long long)p.N * *column_tiles);
-    const long long most = (p.S + (long long)kBatch * p.row_lanes - 1) / ((long long)kBatch * p.row_lanes);
-    if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
-    p.rows = (p.S + splits - 1) / splits;
-    p.splits = (int)((p.S + p.rows - 1) / p.rows);
+    const long long tiles = (words + kThreads - 1) / kThreads;
+    s.words = (int)((words + tiles - 1) / tiles);
+    s.width = s.words * V;
+    s.slabs = (int)tiles;
+    s.threads = kThreads;
+    s.row_lanes = kThreads / s.words;
+    const int half = (s.row_lanes + 1) / 2;
+    s.parts = s.width >= kThreads ? 1 : kThreads / s.width < half ? kThreads / s.width : half;
+    s.by_words = divisor((uint32_t)s.words);
+    s.by_width = divisor((uint32_t)s.width);
+    long long runs = 148 * 3 / ((long long)p.N * tiles);
+    const long long most = (p.S + 32ll * s.row_lanes - 1) / (32ll * s.row_lanes);
+    if (runs > most) runs = most;
+    if (runs < p.S >> 30) runs = (p.S >> 30) + 1; // a run's rows are counted in 32 bits
+    if (runs < 1) runs = 1;
+    s.rows = (int)((p.S + runs - 1) / runs);
+    s.blocks = (int)((p.S + s.rows - 1) / s.rows);
+    s.shared = sizeof(float2) * (size_t)half * s.width;
+    return s;
 }
 
 Norm describe(const sideaware_group_norm_t& sh, const void* weight, const void* bias) {
@@ -907,12 +1047,13 @@ int word_elements(const sideaware_group_norm_t& sh, uint64_t addresses) {
     return a == 16 ? 16 / e : a >= 4 ? 4 / e : 1;
 }
 
+constexpr int kMostShared = 226 * 1024; // dynamic shared memory of a block
 constexpr int kMaxCluster = 8; // blocks of a cluster that every GPU schedules
 
 // Whether the groups of a sample fit into the shared memory of clusters, and how.  `tensors`: 1 (forward) or 2.  Of every slab
 // width (multiples of the narrowest one that is whole words, up to 512 bytes of a row) and cluster size the one with the least
 // estimated time: rounds of blocks, each with a fixed part (latency, barriers) and its bytes at the SM's share of the HBM.
-bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
+bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     const int most_threads = tensors == 1 ? kResidentThreads : kResidentBackwardThreads, most_blocks = tensors == 1 ? 2 : 3;
     if (p.S > 1 << 20) return false;
     int unit = 1; // groups of the narrowest slab
@@ -947,7 +1088,7 @@ bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
             const size_t data = ((size_t)rows * s.words * V * esize + 15) / 16 * 16;
             s.shared = tensors * data + sizeof(float2) * ((size_t)half * s.width + s.groups + (tensors == 1 ? 0 : 2 * s.width)) +
                        sizeof(float) * (size_t)(tensors == 1 ? 3 : 4) * s.width;
-            if (s.shared > 226 * 1024) continue;
+            if (s.shared > kMostShared) continue;
             const double grid = (double)p.N * s.slabs * blocks;
             if (grid > 1e9) continue;
             int resident = (int)(228 * 1024 / (s.shared + 1024));
@@ -967,12 +1108,65 @@ bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     return least < 1e300;
 }
 
+// The search takes about two microseconds; the last shapes of a thread are looked up instead.
+bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
+    struct Entry {
+        long long S, C;
+        int N, G, V, esize, tensors;
+        bool fits;
+        Slab slab;
+    };
+    constexpr unsigned kEntries = 16;
+    thread_local Entry entries[kEntries] = {};
+    thread_local unsigned next = 0;
+    for (const Entry& e : entries) {
+        if (e.S == p.S && e.C == p.C && e.N == p.N && e.G == p.G && e.V == V && e.esize == esize && e.tensors == tensors) {
+            *best = e.slab;
+            best->p = p;
+            return e.fits;
+        }
+    }
+    Entry& e = entries[next++ % kEntries];
+    e = Entry{p.S, p.C, p.N, p.G, V, esize, tensors, false, Slab{}};
+    e.fits = search_resident(p, V, esize, tensors, &e.slab);
+    *best = e.slab;
+    return e.fits;
+}
+
+// Lets a kernel have more than 48 KiB of dynamic shared memory, once for each kernel and device.
+cudaError_t allow_shared(const void* kernel, size_t bytes) {
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    static std::mutex mu;
+    static std::set<std::pair<const void*, int>> allowed;
+    int device = 0;
+    cudaGetDevice(&device);
+    std::lock_guard<std::mutex> lock(mu);
+    if (allowed.count({kernel, device})) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
+    if (e == cudaSuccess) allowed.insert({kernel, device});
+    return e;
+}
+
+// `follows`: the launch may begin while the previous kernel of the same call ends
+template <class... P, class... Args>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, int threads, size_t shared, bool follows, cudaStream_t stream, Args... args) {
+    if (const cudaError_t e = allow_shared((const void*)kernel, shared); e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = follows && sa_pdl_enabled() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 template <class K, class... Args>
 cudaError_t launch_clusters(K kernel, const Slab& s, cudaStream_t stream, Args... args) {
-    if (s.shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.shared);
-        if (e != cudaSuccess) return e;
-    }
+    if (const cudaError_t e = allow_shared((const void*)kernel, s.shared); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(s.p.N * s.slabs * s.blocks));
     cfg.blockDim = dim3((unsigned)s.threads);
@@ -988,18 +1182,26 @@ cudaError_t launch_clusters(K kernel, const Slab& s, cudaStream_t stream, Args..
 }
 
 template <class T, int V>
+size_t ring_bytes(size_t tile) {
+    const size_t rings = (size_t)kRingWords * kThreads * sizeof(SaVec<T, V>);
+    return rings > tile ? rings : (tile + 15) / 16 * 16;
+}
+
+template <class T, int V>
 cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream) {
     Slab s;
     if (plan_resident(p, V, sizeof(T), 1, &s))
         return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, (T*)out, (const T*)x, mean, rstd, s);
-    int tiles = 0;
-    cut(p, V, &tiles);
-    const dim3 grid((unsigned)p.N * p.splits, tiles);
-    float2* partial = (float2*)workspace;
-    sa_norm_partial_kernel<T, V><<<grid, kThreads, 0, stream>>>((const T*)x, partial, p);
-    sa_norm_join_kernel<<<p.N * p.G, kThreads, 0, stream>>>(partial, mean, rstd, p);
-    sa_norm_apply_kernel<T, V><<<grid, kThreads, 0, stream>>>((T*)out, (const T*)x, mean, rstd, p);
-    return cudaGetLastError();
+    s = cut(p, V);
+    const size_t params = sizeof(float) * 3 * (size_t)s.width;
+    s.shared = ring_bytes<T, V>(s.shared); // stream, then tile; the parameters behind
+    float2* const partial = (float2*)workspace;
+    const unsigned grid = (unsigned)((long long)p.N * s.slabs * s.blocks);
+    cudaError_t e = launch(sa_norm_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)x, partial, s);
+    if (e == cudaSuccess) e = launch(sa_norm_join_kernel, (unsigned)(p.N * p.G), kThreads, 0, true, stream, partial, mean, rstd, s);
+    if (e == cudaSuccess)
+        e = launch(sa_norm_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)out, (const T*)x, mean, rstd, s);
+    return e;
 }
 
 template <class T, int V>
@@ -1011,21 +1213,27 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
         const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
         if (e != cudaSuccess || !sums) return e;
-        sa_norm_backward_params_kernel<<<(unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, stream>>>(sums, dweight, dbias, p);
-        return cudaGetLastError();
+        return launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, false, stream, sums, dweight,
+                      dbias, p);
     }
-    int tiles = 0;
-    cut(p, V, &tiles);
-    const dim3 grid((unsigned)p.N * p.splits, tiles);
-    float2* partial = (float2*)workspace;
-    float2* sums = partial + (long long)p.N * p.splits * p.C;
-    float2* means = sums + (long long)p.N * p.C;
-    sa_norm_backward_partial_kernel<T, V><<<grid, kThreads, 0, stream>>>((const T*)dout, (const T*)x, mean, rstd, partial, p);
-    sa_norm_backward_join_kernel<<<p.N * p.G, kThreads, 0, stream>>>(partial, sums, means, p);
-    if (dweight || dbias)
-        sa_norm_backward_params_kernel<<<(unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, stream>>>(sums, dweight, dbias, p);
-    sa_norm_backward_apply_kernel<T, V><<<grid, kThreads, 0, stream>>>((T*)dx, (const T*)dout, (const T*)x, mean, rstd, means, p);
-    return cudaGetLastError();
+    s = cut(p, V);
+    const unsigned grid = (unsigned)((long long)p.N * s.slabs * s.blocks);
+    const size_t params = sizeof(float) * 5 * (size_t)s.width;
+    s.shared = ring_bytes<T, V>(s.shared); // streams, then tile; the parameters behind
+    float2* const partial = (float2*)workspace;
+    float2* const sums = partial + (long long)p.N * s.blocks * p.C;
+    float2* const means = sums + (long long)p.N * p.C;
+    cudaError_t e = launch(sa_norm_backward_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)dout,
+                           (const T*)x, mean, rstd, partial, s);
+    if (e == cudaSuccess)
+        e = launch(sa_norm_backward_join_kernel, (unsigned)(p.N * p.G), kThreads, 0, true, stream, partial, rstd, sums, means, s);
+    if (e == cudaSuccess)
+        e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)dx, (const T*)dout, (const T*)x, mean,
+                   rstd, means, s);
+    if (e == cudaSuccess && (dweight || dbias))
+        e = launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
+                   dbias, p);
+    return e;
 }
 
 template <class F>
@@ -1055,11 +1263,9 @@ size_t sa_group_norm_workspace(const sideaware_group_norm_t& sh, bool backward) 
         if (sh.C % V) continue;
         Norm p = describe(sh, nullptr, nullptr);
         Slab s;
-        int tiles = 0;
         long long entries = backward && sh.N > 1 ? (long long)sh.N * sh.C : 0;
         if (!plan_resident(p, V, e, backward ? 2 : 1, &s)) {
-            cut(p, V, &tiles);
-            entries = (long long)sh.N * p.splits * sh.C + (backward ? (long long)sh.N * (sh.C + sh.G) : 0);
+            entries = (long long)sh.N * cut(p, V).blocks * sh.C + (backward ? (long long)sh.N * (sh.C + sh.G) : 0);
         }
         if (entries > most) most = entries;
     }

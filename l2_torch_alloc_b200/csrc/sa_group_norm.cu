@@ -17,6 +17,8 @@
 //  * for samples too long for that, three launches: partial statistics of runs of rows, joining them, applying them.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <set>
 #include <type_traits>
@@ -31,11 +33,14 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kResidentThreads = 512, kResidentBackwardThreads = 256; // threads of a resident block, at most
+constexpr int kMaxCluster = 8;                                          // blocks of a cluster that every GPU schedules
+constexpr int kResidentThreads = 512;                                   // threads of a resident block, at most
+constexpr int kResidentRegisters = 64, kResidentBackwardRegisters = 80; // 32 and 25 warps on an SM
 
 struct Norm {
     long long S, C; // rows of a sample, channels
     int G, D;       // groups, channels of a group
+    int fold;       // so many pixels lie side by side in a row: S and C are those of such rows, the operator has C / fold channels
     int N;
     int silu, param_dtype;
     float eps;
@@ -177,12 +182,26 @@ __device__ __forceinline__ F2 sigmoid2(F2 z) {
     return f2(r, r) * f2(y, x);
 }
 
-// dy act'(z)
-template <class T>
-__device__ __forceinline__ F2 through_activation2(F2 dy, F2 z, int silu) {
-    if (!silu) return dy;
+// The inner loops exist with and without the activation, which is one branch around them: with_activation(silu, f) calls
+// f(std::true_type) or f(std::false_type).
+template <class F>
+__device__ __forceinline__ void with_activation(int silu, F&& f) {
+    if (silu) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+template <class T, bool SILU>
+__device__ __forceinline__ F2 activation2(F2 z) {
+    if constexpr (!SILU) return z;
+    return z * sigmoid2<T>(z);
+}
+
+// dy act'(z) = dy s (1 + z (1 - s))
+template <class T, bool SILU>
+__device__ __forceinline__ F2 through_activation2(F2 dy, F2 z) {
+    if constexpr (!SILU) return dy;
     const F2 sg = sigmoid2<T>(z), one = f2(1.0f, 1.0f);
-    return dy * (sg * fma2(z, one + negative(sg), one));
+    return dy * (sg * fma2(z, fma2(sg, f2(-1.0f, -1.0f), one), one));
 }
 
 // A channel's row lanes, `parts` threads for each channel; the sum stands in the first row of each share.
@@ -190,11 +209,13 @@ __device__ __forceinline__ void column_sums(const Slab& s, int lanes, float2* ti
     for (int j = threadIdx.x; j < s.parts * s.width; j += blockDim.x) {
         const int part = s.parts > 1 ? (int)s.by_width.div(j) : 0; // j = part * width + channel
         float2 t = tile[j];
-        const float2* e = tile + j;
+        const float2* at = tile + j;
+#pragma unroll 4
         for (int r = part + s.parts; r < lanes; r += s.parts) {
-            e += s.parts * s.width;
-            t.x += e->x;
-            t.y += e->y;
+            at += s.parts * s.width;
+            const float2 e = *at;
+            t.x += e.x;
+            t.y += e.y;
         }
         tile[j] = t;
     }
@@ -215,12 +236,18 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// the operator's channel at place c of a row
+__device__ __forceinline__ long long channel_of(const Norm& p, long long c) {
+    return p.fold > 1 ? (long long)((uint32_t)c % ((uint32_t)p.C / (uint32_t)p.fold)) : c;
+}
+
 // weight and bias of the slab's channels (1 and 0 where there are none) into shared memory, without a barrier
 __device__ __forceinline__ void stage_params(const Slab& s, const Place& w, float* weight, float* bias) {
     for (int j = threadIdx.x; j < s.width; j += blockDim.x) {
         const bool is = j < w.channels;
-        weight[j] = is && s.p.weight ? sa_param(s.p.weight, w.first + j, s.p.param_dtype) : 1.0f;
-        bias[j] = is && s.p.bias ? sa_param(s.p.bias, w.first + j, s.p.param_dtype) : 0.0f;
+        const long long c = channel_of(s.p, w.first + j);
+        weight[j] = is && s.p.weight ? sa_param(s.p.weight, c, s.p.param_dtype) : 1.0f;
+        bias[j] = is && s.p.bias ? sa_param(s.p.bias, c, s.p.param_dtype) : 0.0f;
     }
 }
 
@@ -302,6 +329,7 @@ template <int V>
 __device__ __forceinline__ float2 channel_sum(const Slab& s, const float2* tile, int c) {
     const float2* const at = tile + tile_place<V>(s, c);
     float2 t = *at;
+#pragma unroll 4
     for (int part = 1; part < s.parts; ++part) {
         const float2 e = at[part * s.width];
         t.x += e.x;
@@ -376,7 +404,41 @@ __device__ __forceinline__ void stream_rows(int rows, Fetch&& fetch, Stage&& sta
 __device__ __forceinline__ void may_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// partial[n][run][c] = (mean, m2) of channel c over the run's rows
+// The groups that a slab touches: with folded rows (one slab) all of them.
+__device__ __forceinline__ int first_group(const Norm& p, long long first) { return p.fold > 1 ? 0 : (int)((uint32_t)first / (uint32_t)p.D); }
+__device__ __forceinline__ int last_group(const Norm& p, long long first, int channels) {
+    return p.fold > 1 ? p.G - 1 : (int)((uint32_t)(first + channels - 1) / (uint32_t)p.D);
+}
+// Lanes that work on a group together: the power of two that its places of a slab keep busy.
+__device__ __forceinline__ int group_lanes(const Norm& p) {
+    const int places = p.D * p.fold;
+    return places > 16 ? 32 : places > 8 ? 16 : places > 4 ? 8 : 4;
+}
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// f(g, whether there is such a group) for the groups g0 to g1, `lanes` threads for each; all threads of a warp call f together
+template <class F>
+__device__ __forceinline__ void for_groups(int g0, int g1, int lanes, F&& f) {
+    const int at_once = kThreads / lanes;
+    for (int g = g0; g <= g1; g += at_once) {
+        const int mine = g + (int)threadIdx.x / lanes;
+        f(min(mine, g1), mine <= g1);
+    }
+}
+// f(j) for this lane's share of the places j of group g in a slab
+template <class F>
+__device__ __forceinline__ void for_group(const Norm& p, long long first, int channels, int g, int lanes, F&& f) {
+    const long long each = p.C / p.fold;
+    for (int copy = 0; copy < p.fold; ++copy) {
+        const long long base = copy * each - first;
+        const long long from = max((long long)g * p.D, -base), end = min((long long)(g + 1) * p.D, channels - base);
+        for (long long c = from + (threadIdx.x & (lanes - 1)); c < end; c += lanes) f((int)(base + c));
+    }
+}
+
+// partial[n][run][slab][group of the slab] = (mean, m2) of the group's channels in the slab over the run's rows
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, 3)
 sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, const __grid_constant__ Slab s) {
@@ -435,12 +497,34 @@ sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, co
     __syncthreads();
     refer_to_centre<V>(w, m, q, n, centre);
     block_sums<V>(s, w, tile, m, q);
+    // the channels' means and squared deviations, then some lanes for each group: equally many values in each channel
+    float* const deviation = centre + s.width;
     const float rows_inv = w.block_rows > 0 ? 1.0f / (float)w.block_rows : 0.0f;
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
         const float2 t = channel_sum<V>(s, tile, j);
         const float off = t.x * rows_inv;
-        partial[((long long)w.n * s.blocks + w.rank) * p.C + w.first + j] = make_float2(centre[j] + off, fmaf(-t.x, off, t.y));
+        centre[j] += off;
+        deviation[j] = fmaf(-t.x, off, t.y);
     }
+    __syncthreads();
+    const int g0 = first_group(p, w.first), g1 = last_group(p, w.first, w.channels);
+    float2* const to = partial + (((long long)w.n * s.blocks + w.rank) * s.slabs + w.first / s.width) * s.groups;
+    const int lanes = group_lanes(p);
+    for_groups(g0, g1, lanes, [&](int g, bool is) {
+        float n_channels = 0.0f, sum = 0.0f, m2 = 0.0f;
+        for_group(p, w.first, w.channels, g, lanes, [&](int j) {
+            n_channels += 1.0f;
+            sum += centre[j];
+            m2 += deviation[j];
+        });
+        const float mg = __fdividef(lanes_sum(sum, lanes), lanes_sum(n_channels, lanes));
+        for_group(p, w.first, w.channels, g, lanes, [&](int j) {
+            const float off = centre[j] - mg;
+            m2 = fmaf(off * off, (float)w.block_rows, m2);
+        });
+        m2 = lanes_sum(m2, lanes);
+        if (is && (threadIdx.x & (lanes - 1)) == 0) to[g - g0] = make_float2(mg, m2);
+    });
 }
 
 // mean and rstd of (n, g): one block each
@@ -450,20 +534,19 @@ sa_norm_join_kernel(const float2* __restrict__ partial, float* __restrict__ mean
     may_follow();
     const Norm& p = s.p;
     const uint32_t n = blockIdx.x / (uint32_t)p.G, g = blockIdx.x - n * (uint32_t)p.G;
-    // some threads for each channel, each a share of the runs; channels beyond the block's width in turn
-    const int wide = min(p.D, kThreads), shares = kThreads / wide;
-    const int share = threadIdx.x / wide, lane = threadIdx.x - share * wide;
     const float last = (float)(p.S - (long long)(s.blocks - 1) * s.rows);
+    const uint32_t c0 = g * (uint32_t)p.D, c1 = c0 + (uint32_t)p.D; // the group's channels lie in slabs t0 to t1
+    const uint32_t t0 = p.fold > 1 ? 0 : c0 / (uint32_t)s.width, t1 = p.fold > 1 ? 0 : (c1 - 1) / (uint32_t)s.width;
     Moments m{0.0f, 0.0f, 0.0f};
     await_previous();
-    if (share < shares) {
-        for (int d = lane; d < p.D; d += wide) {
-            const float2* const from = partial + (long long)n * s.blocks * p.C + (long long)g * p.D + d;
-#pragma unroll 8
-            for (int r = share; r < s.blocks; r += shares) {
-                const float2 e = from[(long long)r * p.C];
-                join(m, Moments{r + 1 == s.blocks ? last : (float)s.rows, e.x, e.y});
-            }
+    for (uint32_t t = t0; t <= t1; ++t) {
+        const uint32_t first = t * (uint32_t)s.width;
+        const float channels = p.fold > 1 ? (float)p.D * (float)p.fold : (float)(min(c1, first + (uint32_t)s.width) - max(c0, first));
+        const float2* const from = partial + ((long long)n * s.blocks * s.slabs + t) * s.groups + (g - first_group(p, first));
+#pragma unroll 4
+        for (int r = threadIdx.x; r < s.blocks; r += kThreads) {
+            const float2 e = from[(long long)r * s.slabs * s.groups];
+            join(m, Moments{(r + 1 == s.blocks ? last : (float)s.rows) * channels, e.x, e.y});
         }
     }
     m = warp_join(m);
@@ -493,7 +576,7 @@ sa_norm_apply_kernel(T* out, const T* x, const float* __restrict__ mean, const f
     stage_params(s, w, weight, bias);
     await_previous();
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
-        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        const long long at = (long long)w.n * p.G + (uint32_t)channel_of(p, w.first + j) / (uint32_t)p.D;
         centre[j] = mean[at];
         weight[j] *= rstd[at];
     }
@@ -509,18 +592,17 @@ sa_norm_apply_kernel(T* out, const T* x, const float* __restrict__ mean, const f
     const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V + (w.rows - 1) * step;
     Stream<T, V> in(memory, x + base, -step);
     T* to = out + base;
-    stream_rows<kRingWords / kStreamStages>(
-        w.rows, [&](int slot) { in.fetch(slot); }, [](int, int) {},
-        [&](int slot) {
-            SaVec<T, V> v = in.row(slot);
+    with_activation(p.silu, [&](auto silu) {
+        stream_rows<kRingWords / kStreamStages>(
+            w.rows, [&](int slot) { in.fetch(slot); }, [](int, int) {},
+            [&](int slot) {
+                SaVec<T, V> v = in.row(slot);
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const F2 z = fma2(pair_of(v, k) + m[k], a[k], b[k]);
-                set_pair(v, k, p.silu ? z * sigmoid2<T>(z) : z);
-            }
-            sa_store_stream<T, V>(to, v);
-            to -= step;
-        });
+                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], b[k])));
+                sa_store_stream<T, V>(to, v);
+                to -= step;
+            });
+    });
 }
 
 // partial[n][run][c] = (sum dz, sum dz (x - mean)) over the run's rows
@@ -541,7 +623,7 @@ sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict_
     const Norm& p = s.p;
     stage_params(s, w, slope, bias);
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
-        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        const long long at = (long long)w.n * p.G + (uint32_t)channel_of(p, w.first + j) / (uint32_t)p.D;
         centre[j] = mean[at];
         slope[j] *= rstd[at];
     }
@@ -560,81 +642,62 @@ sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict_
     const long long step = (long long)s.row_lanes * p.C;
     const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V;
     Stream<T, V> in(memory, x + base, step), grad(memory + kRing, dout + base, step);
-    stream_rows<kRows>(
-        w.rows,
-        [&](int slot) {
-            in.fetch(slot);
-            grad.fetch(slot);
-        },
-        [](int, int) {},
-        [&](int slot) {
-            const SaVec<T, V> v = in.row(slot), d = grad.row(slot);
+    with_activation(p.silu, [&](auto silu) {
+        stream_rows<kRows>(
+            w.rows,
+            [&](int slot) {
+                in.fetch(slot);
+                grad.fetch(slot);
+            },
+            [](int, int) {},
+            [&](int slot) {
+                const SaVec<T, V> v = in.row(slot), d = grad.row(slot);
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const F2 dev = pair_of(v, k) + m[k];
-                const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
-                a0[k] = a0[k] + dz;
-                a1[k] = fma2(dz, dev, a1[k]);
-            }
-        });
+                for (int k = 0; k < P; ++k) {
+                    const F2 dev = pair_of(v, k) + m[k];
+                    const F2 dz = through_activation2<T, silu.value>(pair_of(d, k), fma2(dev, sl[k], b[k]));
+                    a0[k] = a0[k] + dz;
+                    a1[k] = fma2(dz, dev, a1[k]);
+                }
+            });
+    });
     __syncthreads(); // the rings become the tile
     block_sums<V>(s, w, tile, a0, a1);
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x)
         partial[((long long)w.n * s.blocks + w.rank) * p.C + w.first + j] = channel_sum<V>(s, tile, j);
 }
 
-// sums[n][c] = (sum dz, sum dz u), and of every (n, g) (-rstd m1, -rstd^2 m2): one block for each (n, g)
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_join_kernel(const float2* __restrict__ partial, const float* __restrict__ rstd, float2* __restrict__ sums,
-                             float2* __restrict__ means, const __grid_constant__ Slab s) {
-    __shared__ float2 tile[kThreads];
+// sums[n][c] = (sum dz, sum dz u): a block for 32 channels of a sample, 32 shares of the runs
+__global__ void __launch_bounds__(1024)
+sa_norm_backward_sums_kernel(const float2* __restrict__ partial, const float* __restrict__ rstd, float2* __restrict__ sums, const __grid_constant__ Slab s) {
+    __shared__ float2 tile[32][33];
     may_follow();
-    await_previous();
     const Norm& p = s.p;
-    const uint32_t n = blockIdx.x / (uint32_t)p.G, g = blockIdx.x - n * (uint32_t)p.G;
-    const float rs = rstd[blockIdx.x];
-    // some threads for each channel, each a share of the runs; channels beyond the block's width in turn
-    const int wide = min(p.D, kThreads), shares = kThreads / wide;
-    const int share = threadIdx.x / wide, lane = threadIdx.x - share * wide;
-    float2 m = make_float2(0.0f, 0.0f);
-    for (int d0 = 0; d0 < p.D; d0 += wide) {
-        const long long c = (long long)g * p.D + d0 + lane;
-        const bool mine = d0 + lane < p.D && share < shares;
-        float2 t = make_float2(0.0f, 0.0f);
-        if (mine) {
+    const long long channels = p.C / p.fold;
+    const uint32_t tiles = (uint32_t)((channels + 31) / 32), n = blockIdx.x / tiles;
+    const long long c = (long long)(blockIdx.x - n * tiles) * 32 + threadIdx.x % 32;
+    const int share = threadIdx.x / 32;
+    float2 t = make_float2(0.0f, 0.0f);
+    await_previous();
+    if (c < channels) {
+        for (int copy = 0; copy < p.fold; ++copy) { // the pixels side by side
+            const float2* const from = partial + (long long)n * s.blocks * p.C + copy * channels + c;
 #pragma unroll 4
-            for (int r = share; r < s.blocks; r += shares) {
-                const float2 e = partial[((long long)n * s.blocks + r) * p.C + c];
+            for (int r = share; r < s.blocks; r += 32) {
+                const float2 e = from[(long long)r * p.C];
                 t.x += e.x;
                 t.y += e.y;
             }
         }
-        tile[threadIdx.x] = t;
-        __syncthreads();
-        if (mine && share == 0) {
-            for (int q = 1; q < shares; ++q) {
-                t.x += tile[q * wide + lane].x;
-                t.y += tile[q * wide + lane].y;
-            }
-            t.y *= rs;
-            sums[(long long)n * p.C + c] = t;
-            const float w = p.weight ? sa_param(p.weight, c, p.param_dtype) : 1.0f;
-            m.x = fmaf(w, t.x, m.x);
-            m.y = fmaf(w, t.y, m.y);
-        }
-        __syncthreads();
     }
-    m = make_float2(warp_sum(m.x), warp_sum(m.y));
-    if (threadIdx.x % 32 == 0) tile[threadIdx.x / 32] = m;
+    tile[share][threadIdx.x % 32] = t;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < kThreads / 32; ++k) {
-            m.x += tile[k].x;
-            m.y += tile[k].y;
-        }
-        const float inv = 1.0f / ((float)p.S * (float)p.D);
-        means[blockIdx.x] = make_float2(-rs * (m.x * inv), -rs * (m.y * inv) * rs);
-    }
+    // warp w adds up channel w of the 32
+    t = tile[threadIdx.x % 32][share];
+    t = make_float2(warp_sum(t.x), warp_sum(t.y));
+    const long long mine = (long long)(blockIdx.x - n * tiles) * 32 + share;
+    if (threadIdx.x % 32 == 0 && mine < channels)
+        sums[(long long)n * channels + mine] = make_float2(t.x, t.y * rstd[(long long)n * p.G + (uint32_t)mine / (uint32_t)p.D]);
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -656,7 +719,7 @@ sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, 3)
 sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
-                              const float2* __restrict__ means, const __grid_constant__ Slab s) {
+                              const float2* __restrict__ sums, const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     extern __shared__ __align__(16) unsigned char memory[];
     constexpr int kRows = kRingWords / 2 / kStreamStages;
@@ -672,13 +735,47 @@ sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __r
     stage_params(s, w, slope, bias);
     await_previous();
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
-        const long long at = (long long)w.n * p.G + (uint32_t)(w.first + j) / (uint32_t)p.D;
+        const long long at = (long long)w.n * p.G + (uint32_t)channel_of(p, w.first + j) / (uint32_t)p.D;
         centre[j] = mean[at];
         slope[j] *= rstd[at];
-        const float2 e = means[at];
-        first[j] = e.x;
-        second[j] = e.y;
     }
+    // -rstd m1 and -rstd^2 m2 of the groups, from the sums of all their channels: these are in this slab (and come through
+    // shared memory), unless there are several slabs
+    const long long each = p.C / p.fold;
+    const float2* const of_sample = sums + (long long)w.n * each;
+    auto weighted = [&](long long c) {
+        const float wc = p.weight ? sa_param(p.weight, c, p.param_dtype) : 1.0f;
+        const float2 e = of_sample[c];
+        return make_float2(wc * e.x, wc * e.y);
+    };
+    if (s.slabs == 1) {
+        for (int j = threadIdx.x; j < (int)each; j += kThreads) {
+            const float2 e = weighted(j);
+            first[j] = e.x;
+            second[j] = e.y;
+        }
+        __syncthreads();
+    }
+    const float inv = 1.0f / ((float)p.S * (float)p.fold * (float)p.D);
+    const int lanes = s.slabs == 1 ? group_lanes(p) : 32;
+    for_groups(first_group(p, w.first), last_group(p, w.first, w.channels), lanes, [&](int g, bool is) {
+        float2 t = make_float2(0.0f, 0.0f);
+        for (int d = threadIdx.x & (lanes - 1); d < p.D; d += lanes) {
+            const int c = g * p.D + d;
+            const float2 e = s.slabs == 1 ? make_float2(first[c], second[c]) : weighted(c);
+            t.x += e.x;
+            t.y += e.y;
+        }
+        const float rs = rstd[(long long)w.n * p.G + g];
+        const float m1 = -rs * (lanes_sum(t.x, lanes) * inv), m2 = -rs * (lanes_sum(t.y, lanes) * inv) * rs;
+        __syncwarp(); // every lane of the group has read its channels
+        if (is)
+            for_group(p, w.first, w.channels, g, lanes, [&](int j) {
+                first[j] = m1;
+                second[j] = m2;
+            });
+        __syncwarp();
+    });
     __syncthreads();
     if (w.rows <= 0) return;
     F2 m[P], sl[P], b[P], m1[P], m2[P];
@@ -693,25 +790,27 @@ sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __r
     const long long base = ((long long)w.n * p.S + (long long)w.rank * s.rows + w.row_lane) * p.C + w.first + w.word * V + (w.rows - 1) * step;
     Stream<T, V> in(memory, x + base, -step), grad(memory + kRing, dout + base, -step);
     T* to = dx + base;
-    stream_rows<kRows>(
-        w.rows,
-        [&](int slot) {
-            in.fetch(slot);
-            grad.fetch(slot);
-        },
-        [](int, int) {},
-        [&](int slot) {
-            SaVec<T, V> v = in.row(slot);
-            const SaVec<T, V> d = grad.row(slot);
+    with_activation(p.silu, [&](auto silu) {
+        stream_rows<kRows>(
+            w.rows,
+            [&](int slot) {
+                in.fetch(slot);
+                grad.fetch(slot);
+            },
+            [](int, int) {},
+            [&](int slot) {
+                SaVec<T, V> v = in.row(slot);
+                const SaVec<T, V> d = grad.row(slot);
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const F2 dev = pair_of(v, k) + m[k];
-                const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
-                set_pair(v, k, fma2(dev, m2[k], fma2(sl[k], dz, m1[k])));
-            }
-            sa_store_stream<T, V>(to, v);
-            to -= step;
-        });
+                for (int k = 0; k < P; ++k) {
+                    const F2 dev = pair_of(v, k) + m[k];
+                    const F2 dz = through_activation2<T, silu.value>(pair_of(d, k), fma2(dev, sl[k], b[k]));
+                    set_pair(v, k, fma2(dev, m2[k], fma2(sl[k], dz, m1[k])));
+                }
+                sa_store_stream<T, V>(to, v);
+                to -= step;
+            });
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -722,7 +821,7 @@ sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __r
 // their sums to the mean of row lane 0 (the same argument, with its rows among the block's), which makes them plain sums;
 // the channels of a group have equally many values, and the blocks of a cluster are joined by Chan's rule.
 template <class T, int V>
-__global__ void __launch_bounds__(kResidentThreads, 2)
+__global__ void __maxnreg__(kResidentRegisters)
 sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     extern __shared__ __align__(16) unsigned char memory[];
@@ -770,7 +869,8 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
         }
     });
     if (w.rows > 0) {
-        const F2 inv = f2(1.0f / n, 1.0f / n);
+        const float share = __fdividef(1.0f, n);
+        const F2 inv = f2(share, share);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
             const F2 part = m[k] * inv;
@@ -782,50 +882,54 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
     __syncthreads();
     refer_to_centre<V>(w, m, q, n, centre);
     block_sums<V>(s, w, tile, m, q);
-    // a warp for each group
-    const float rows_inv = w.block_rows > 0 ? 1.0f / (float)w.block_rows : 0.0f, D_inv = 1.0f / (float)p.D;
-    for (int g = threadIdx.x / 32; g < w.groups; g += blockDim.x / 32) {
+    // a warp for each group: its channels, then the blocks of the cluster (lane r has block r), then the channels' constants
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+    const float rows_inv = w.block_rows > 0 ? __fdividef(1.0f, (float)w.block_rows) : 0.0f, D_inv = __fdividef(1.0f, (float)p.D);
+    auto finish = [&](int g, float mg, float m2, float count) { // all lanes have the group's moments
+        const float rs = 1.0f / sqrtf(m2 / count + p.eps);
+        for (int d = lane; d < p.D; d += 32) {
+            centre[g * p.D + d] = mg;
+            weight[g * p.D + d] *= rs;
+        }
+        if (w.rank == 0 && lane == 0) {
+            const long long at = (long long)w.n * p.G + w.group0 + g;
+            mean[at] = mg;
+            rstd[at] = rs;
+        }
+    };
+    for (int g = warp; g < w.groups; g += warps) {
         float sum = 0.0f, m2 = 0.0f;
-        for (int d = threadIdx.x % 32; d < p.D; d += 32) { // a channel's mean and squared deviations
+        for (int d = lane; d < p.D; d += 32) { // a channel's mean and squared deviations
             const int c = g * p.D + d;
             const float2 t = channel_sum<V>(s, tile, c);
             const float off = t.x * rows_inv, mc = centre[c] + off;
-            tile[tile_place<V>(s, c)].x = mc;
+            centre[c] = mc;
             m2 += fmaf(-t.x, off, t.y);
             sum += mc;
         }
         const float mg = warp_sum(sum) * D_inv;
-        for (int d = threadIdx.x % 32; d < p.D; d += 32) {
-            const float off = tile[tile_place<V>(s, g * p.D + d)].x - mg; // written by this lane
+        for (int d = lane; d < p.D; d += 32) {
+            const float off = centre[g * p.D + d] - mg; // written by this lane
             m2 = fmaf(off * off, (float)w.block_rows, m2);
         }
         m2 = warp_sum(m2);
-        if (threadIdx.x % 32 == 0) joined[g] = make_float2(mg, m2);
+        if (s.blocks == 1) finish(g, mg, m2, (float)w.block_rows * (float)p.D);
+        else if (lane == 0) joined[g] = make_float2(mg, m2);
     }
 
     cg::cluster_group cluster = cg::this_cluster();
-    if (s.blocks > 1) cluster.sync();
-    else __syncthreads();
-    for (int j = threadIdx.x; j < w.channels; j += blockDim.x) { // every channel joins its group's blocks
-        const int g = (int)s.by_D.div(j);
-        Moments t{0.0f, 0.0f, 0.0f};
-        if (s.blocks == 1) {
-            t = Moments{(float)w.block_rows * (float)p.D, joined[g].x, joined[g].y};
-        } else {
-            int left = (int)p.S;
-#pragma unroll 4
-            for (int r = 0; r < s.blocks; ++r, left -= s.rows) {
-                const float2 e = *cluster.map_shared_rank(joined + g, r);
-                join(t, Moments{(float)max(0, min(left, s.rows)) * (float)p.D, e.x, e.y});
+    if (s.blocks > 1) {
+        cluster.sync();
+        for (int g = warp; g < w.groups; g += warps) {
+            Moments t{0.0f, 0.0f, 0.0f};
+            if (lane < s.blocks) {
+                const float2 e = *cluster.map_shared_rank(joined + g, lane);
+                t = Moments{(float)max(0, min((int)p.S - lane * s.rows, s.rows)) * (float)p.D, e.x, e.y};
             }
-        }
-        const float rs = 1.0f / sqrtf(t.m2 / t.n + p.eps);
-        centre[j] = t.mean;
-        weight[j] *= rs;
-        if (w.rank == 0 && j == g * p.D) {
-            const long long at = (long long)w.n * p.G + w.group0 + g;
-            mean[at] = t.mean;
-            rstd[at] = rs;
+#pragma unroll
+            for (int o = kMaxCluster / 2; o > 0; o >>= 1)
+                join(t, Moments{__shfl_down_sync(0xffffffffu, t.n, o), __shfl_down_sync(0xffffffffu, t.mean, o), __shfl_down_sync(0xffffffffu, t.m2, o)});
+            finish(g, __shfl_sync(0xffffffffu, t.mean, 0), __shfl_sync(0xffffffffu, t.m2, 0), __shfl_sync(0xffffffffu, t.n, 0));
         }
     }
     __syncthreads();
@@ -837,17 +941,17 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
         shared_pairs<V>(b, bias + w.word * V);
 #pragma unroll
         for (int k = 0; k < P; ++k) m[k] = negative(m[k]);
-        T* to = out + base;
+        with_activation(p.silu, [&](auto silu) {
+            T* to = out + base;
+            const SaVec<T, V>* row = mine;
 #pragma unroll 2
-        for (int u = 0; u < w.rows; ++u, to += step) {
-            SaVec<T, V> v = mine[u * stride];
+            for (int u = 0; u < w.rows; ++u, to += step, row += stride) {
+                SaVec<T, V> v = *row;
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const F2 z = fma2(pair_of(v, k) + m[k], a[k], b[k]);
-                set_pair(v, k, p.silu ? z * sigmoid2<T>(z) : z);
+                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], b[k])));
+                sa_store<T, V>(to, v);
             }
-            sa_store<T, V>(to, v);
-        }
+        });
     }
     if (s.blocks > 1) cluster.barrier_wait(); // no block leaves while a neighbour may still read its shared memory
 }
@@ -856,7 +960,7 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
 //   z = (x - mean) (w rstd) + b,  dx = (w rstd) dz - rstd m1 - (x - mean) rstd^2 m2
 // `sums`: (sum dz, sum dz u) of every (n, c); NULL: there is one sample, dweight and dbias are written here
 template <class T, int V>
-__global__ void __launch_bounds__(kResidentBackwardThreads, 3)
+__global__ void __maxnreg__(kResidentBackwardRegisters)
 sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
                                  float2* __restrict__ sums, void* __restrict__ dweight, void* __restrict__ dbias,
                                  const __grid_constant__ Slab s) {
@@ -873,6 +977,7 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
     float* const bias = weight + s.width;
     float* const centre = bias + s.width;
     float* const slope = centre + s.width; // weight * rstd
+    may_follow();
     const Place w = place_of<V>(s, blockIdx.x);
     const Norm& p = s.p;
 
@@ -910,17 +1015,21 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
 #pragma unroll
             for (int k = 0; k < P; ++k) m[k] = negative(m[k]);
         }
-        as_rows_arrive(w.rows, [&](int u, int end) {
-            for (; u < end; ++u) {
-                const SaVec<T, V> v = mine[u * stride], d = theirs[u * stride];
+        with_activation(p.silu, [&](auto silu) {
+            as_rows_arrive(w.rows, [&](int u, int end) {
+                const SaVec<T, V>*row = mine + u * stride, *other = theirs + u * stride;
+#pragma unroll 2
+                for (; u < end; ++u, row += stride, other += stride) {
+                    const SaVec<T, V> v = *row, d = *other;
 #pragma unroll
-                for (int k = 0; k < P; ++k) {
-                    const F2 dev = pair_of(v, k) + m[k];
-                    const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
-                    a0[k] = a0[k] + dz;
-                    a1[k] = fma2(dz, dev, a1[k]);
+                    for (int k = 0; k < P; ++k) {
+                        const F2 dev = pair_of(v, k) + m[k];
+                        const F2 dz = through_activation2<T, silu.value>(pair_of(d, k), fma2(dev, sl[k], b[k]));
+                        a0[k] = a0[k] + dz;
+                        a1[k] = fma2(dz, dev, a1[k]);
+                    }
                 }
-            }
+            });
         });
         block_sums<V>(s, w, tile, a0, a1);
     }
@@ -929,12 +1038,17 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
     if (s.blocks > 1) cluster.sync();
     else __syncthreads();
     for (int j = threadIdx.x; j < w.channels; j += blockDim.x) {
-        float2 t = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-        for (int r = 0; r < s.blocks; ++r) {
-            const float2 e = s.blocks > 1 ? *cluster.map_shared_rank(channel + j, r) : channel[j];
-            t.x += e.x;
-            t.y += e.y;
+        float2 t = channel[j];
+        if (s.blocks > 1) {
+            t = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) { // all in flight together
+                if (r < s.blocks) {
+                    const float2 e = *cluster.map_shared_rank(channel + j, r);
+                    t.x += e.x;
+                    t.y += e.y;
+                }
+            }
         }
         total[j] = make_float2(weight[j] * t.x, slope[j] * t.y);
         t.y *= means[s.by_D.div(j)].x; // sum of dz u
@@ -967,11 +1081,16 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
         F2 m1[P], m2[P];
         {
             float x1[2 * P] = {}, x2[2 * P] = {};
+            int g = (int)s.by_D.div(w.word * V), r = w.word * V - g * p.D;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float2 e = means[s.by_D.div(w.word * V + i)];
+                const float2 e = means[g];
                 x1[i] = e.x;
                 x2[i] = e.y;
+                if (++r == p.D) {
+                    r = 0;
+                    ++g;
+                }
             }
 #pragma unroll
             for (int k = 0; k < P; ++k) {
@@ -979,18 +1098,22 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
                 m2[k] = f2(x2[2 * k], x2[2 * k + 1]);
             }
         }
-        T* to = dx + base;
-        for (int u = 0; u < w.rows; ++u, to += step) {
-            SaVec<T, V> v = mine[u * stride];
-            const SaVec<T, V> d = theirs[u * stride];
+        with_activation(p.silu, [&](auto silu) {
+            T* to = dx + base;
+            const SaVec<T, V>*row = mine, *other = theirs;
+#pragma unroll 2
+            for (int u = 0; u < w.rows; ++u, to += step, row += stride, other += stride) {
+                SaVec<T, V> v = *row;
+                const SaVec<T, V> d = *other;
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const F2 dev = pair_of(v, k) + m[k];
-                const F2 dz = through_activation2<T>(pair_of(d, k), fma2(dev, sl[k], b[k]), p.silu);
-                set_pair(v, k, fma2(dev, m2[k], fma2(sl[k], dz, m1[k])));
+                for (int k = 0; k < P; ++k) {
+                    const F2 dev = pair_of(v, k) + m[k];
+                    const F2 dz = through_activation2<T, silu.value>(pair_of(d, k), fma2(dev, sl[k], b[k]));
+                    set_pair(v, k, fma2(dev, m2[k], fma2(sl[k], dz, m1[k])));
+                }
+                sa_store<T, V>(to, v);
             }
-            sa_store<T, V>(to, v);
-        }
+        });
     }
     if (s.blocks > 1) cluster.barrier_wait(); // no block leaves while a neighbour may still read its shared memory
 }
@@ -998,6 +1121,14 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
+// Threads that share a channel's column of `lanes` values: the column is added up in lanes / shares steps, the shares in
+// `shares` steps, so the square root is best.
+int shares(int lanes, int most) {
+    int n = 1;
+    while (n < most && n * n < lanes) ++n;
+    return n;
+}
+
 // Samples too long to be resident: words across a block, rows at a time, runs of rows.  Three blocks for each SM, but runs
 // of at least 32 rows for each row lane, so that partial results stay a small part of the traffic.
 Slab cut(const Norm& p, int V) {
@@ -1011,7 +1142,7 @@ Slab cut(const Norm& p, int V) {
     s.threads = kThreads;
     s.row_lanes = kThreads / s.words;
     const int half = (s.row_lanes + 1) / 2;
-    s.parts = s.width >= kThreads ? 1 : kThreads / s.width < half ? kThreads / s.width : half;
+    s.parts = shares(half, kThreads / s.width);
     s.by_words = divisor((uint32_t)s.words);
     s.by_width = divisor((uint32_t)s.width);
     long long runs = 148 * 3 / ((long long)p.N * tiles);
@@ -1022,6 +1153,7 @@ Slab cut(const Norm& p, int V) {
     s.rows = (int)((p.S + runs - 1) / runs);
     s.blocks = (int)((p.S + s.rows - 1) / s.rows);
     s.shared = sizeof(float2) * (size_t)half * s.width;
+    s.groups = p.fold > 1 || s.width / p.D + 2 > p.G ? p.G : s.width / p.D + 2; // that a slab touches, at most
     return s;
 }
 
@@ -1032,6 +1164,7 @@ Norm describe(const sideaware_group_norm_t& sh, const void* weight, const void* 
     p.C = sh.C;
     p.G = sh.G;
     p.D = sh.C / sh.G;
+    p.fold = 1;
     p.silu = sh.silu;
     p.param_dtype = sh.param_dtype;
     p.eps = sh.eps;
@@ -1040,29 +1173,54 @@ Norm describe(const sideaware_group_norm_t& sh, const void* weight, const void* 
     return p;
 }
 
-// elements of a word: 16 bytes where addresses and rows allow them, else 4, else one element
-int word_elements(const sideaware_group_norm_t& sh, uint64_t addresses) {
-    const int e = sa_element_size(sh.dtype);
-    const int a = sa_common_alignment(addresses | (uint64_t)sh.C * (uint64_t)e);
-    return a == 16 ? 16 / e : a >= 4 ? 4 / e : 1;
-}
 
 constexpr int kMostShared = 226 * 1024; // dynamic shared memory of a block
-constexpr int kMaxCluster = 8; // blocks of a cluster that every GPU schedules
 
-// Whether the groups of a sample fit into the shared memory of clusters, and how.  `tensors`: 1 (forward) or 2.  Of every slab
-// width (multiples of the narrowest one that is whole words, up to 512 bytes of a row) and cluster size the one with the least
-// estimated time: rounds of blocks, each with a fixed part (latency, barriers) and its bytes at the SM's share of the HBM.
+// How a resident launch would run, in microseconds.  The form is a sum of what an SM has to do in each round of blocks; the
+// constants were fitted to 2,600 measured launches (26 shapes, forward and backward, all slab widths, cluster sizes and block
+// sizes) with a mean error of 14 %: the choice that follows from it took 4 % longer than each shape's best one.
+double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors) {
+    // blocks that run at once when each has an SM (or a share of one) to itself: a cluster stays inside a GPC, so sizes that
+    // do not divide a GPC's SMs leave some idle (cudaOccupancyMaxActiveClusters)
+    static const int kAlone[kMaxCluster + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+    const int registers = tensors == 1 ? kResidentRegisters : kResidentBackwardRegisters;
+    int on_sm = (int)(228 * 1024 / (s.shared + 1024));
+    if (on_sm > 65536 / (registers * s.threads)) on_sm = 65536 / (registers * s.threads);
+    const double grid = (double)p.N * s.slabs * s.blocks;
+    const double at_once = on_sm == 1 ? kAlone[s.blocks] : 148.0 * on_sm * (s.blocks <= 2 ? 1.0 : 0.92);
+    const double rounds = grid <= at_once ? 1.0 : std::ceil(grid / at_once);
+    const double of_sm = std::min((double)on_sm, std::ceil(grid / 148.0)); // blocks of the busiest SM
+    // memory: segments that do not start and end on sectors, or are shorter than two of them, cost more than their bytes
+    const double segment = (double)s.width * esize, bytes = (double)s.rows * s.words * V * esize;
+    double ragged = (s.width * esize) % 32 ? (segment + 16.0) / segment : 1.0;
+    if (segment < 64.0) ragged *= 2.0 - segment / 64.0;
+    const double memory = of_sm * bytes * (tensors + 1) * ragged / 43e3;
+    // arithmetic: cycles of a warp for a row of its words (V = 8), on four schedulers, fewer than 18 warps do not fill them
+    const double warps = of_sm * s.threads / 32, row = (tensors == 1 ? 34.0 : 214.0) * std::max(V / 8.0, 0.3) * (esize == 4 ? 1.3 : 1.0);
+    const double lanes = std::ceil((double)s.rows / s.row_lanes);
+    const double arithmetic = of_sm * lanes * (s.threads / 32) * row / 4 / 1900 / std::min(1.0, warps / 18.0);
+    const double fixed = 3.0 + (s.blocks > 1 ? 1.0 : 0.0) + 0.4 * s.blocks + (tensors == 1 ? 0.0 : 0.7); // latencies and barriers
+    return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 5.5;
+}
+
+// The same for the way of long samples: three or four launches (fitted to 0.2-134 MB of x; within 20 %).
+double streamed_time(const Norm& p, int V, int esize, int tensors) {
+    const double mb = (double)p.N * (double)p.S * (double)p.C * esize * 1e-6 * (V * esize == 16 ? 1.0 : V * esize == 4 ? 4.0 : 8.0);
+    return tensors == 1 ? 14.6 + 0.48 * mb : 28.0 + 0.75 * mb;
+}
+
+// Whether the groups of a sample are to be resident, and how: every slab width (multiples of the narrowest one that is whole
+// words, up to 512 bytes of a row), cluster size and block size that fits, against each other and against streaming.
 bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
-    const int most_threads = tensors == 1 ? kResidentThreads : kResidentBackwardThreads, most_blocks = tensors == 1 ? 2 : 3;
     if (p.S > 1 << 20) return false;
     int unit = 1; // groups of the narrowest slab
     while ((unit * (long long)p.D) % V) ++unit;
-    double least = 1e300;
-    for (int m = 1; m == 1 || unit * m <= p.G; ++m) {
+    double least = streamed_time(p, V, esize, tensors);
+    bool found = false;
+    for (int m = 1; m == 1 || unit * (m - 1) < p.G; ++m) {
         const int groups = unit * m < p.G ? unit * m : p.G;
         const long long width = (long long)groups * p.D;
-        if (width % V || width / V > most_threads / 2 || (m > 1 && width * esize > 512)) break;
+        if (width % V || width / V > kResidentThreads / 2 || (m > 1 && width * esize > 512)) break;
         Slab s{};
         s.p = p;
         s.groups = groups;
@@ -1072,43 +1230,31 @@ bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
         s.by_words = divisor((uint32_t)s.words);
         s.by_width = divisor((uint32_t)width);
         s.by_D = divisor((uint32_t)p.D);
-        for (int blocks = 1; blocks <= kMaxCluster; ++blocks) {
-            const int rows = (int)((p.S + blocks - 1) / blocks);
-            if (blocks > 1 && rows < 8) break;
-            s.blocks = blocks;
-            s.rows = rows;
-            // about four rows for each thread
-            long long threads = ((long long)rows * s.words / 4 + 31) / 32 * 32;
-            if (threads < 2 * s.words) threads = (2 * s.words + 31) / 32 * 32;
-            if (threads < 128) threads = 128;
-            s.threads = threads > most_threads ? most_threads : (int)threads;
-            s.row_lanes = s.threads / s.words;
-            const int half = (s.row_lanes + 1) / 2;
-            s.parts = s.width >= s.threads ? 1 : s.threads / s.width < half ? s.threads / s.width : half;
-            const size_t data = ((size_t)rows * s.words * V * esize + 15) / 16 * 16;
-            s.shared = tensors * data + sizeof(float2) * ((size_t)half * s.width + s.groups + (tensors == 1 ? 0 : 2 * s.width)) +
-                       sizeof(float) * (size_t)(tensors == 1 ? 3 : 4) * s.width;
-            if (s.shared > kMostShared) continue;
-            const double grid = (double)p.N * s.slabs * blocks;
-            if (grid > 1e9) continue;
-            int resident = (int)(228 * 1024 / (s.shared + 1024));
-            if (resident > most_blocks) resident = most_blocks;
-            const double segment = (double)width * esize, ragged = (width * esize) % 32 ? (segment + 16.0) / segment : 1.0;
-            const double fixed = 2.5 + (blocks > 1 ? 0.7 : 0.0) + 0.1 * blocks;
-            const double bytes = (tensors + 1) * (double)data * ragged / 44e3; // us for one block's traffic at an SM's share
-            const double rounds = grid / (148.0 * resident);
-            const double cost = rounds <= 1.0 ? fixed + bytes * (grid > 148.0 ? resident : 1.0)
-                                              : fixed + (double)(long long)(rounds + 0.999) * (bytes * resident + fixed / resident);
-            if (cost < least) {
-                least = cost;
-                *best = s;
+        for (s.blocks = 1; s.blocks <= kMaxCluster; ++s.blocks) {
+            s.rows = (int)((p.S + s.blocks - 1) / s.blocks);
+            if ((s.blocks > 1 && s.rows < 8) || (double)p.N * s.slabs * s.blocks > 1e9) break;
+            const size_t data = ((size_t)s.rows * s.words * V * esize + 15) / 16 * 16;
+            for (s.threads = 128; s.threads <= kResidentThreads; s.threads += 128) {
+                if (s.threads < 2 * s.words) continue;
+                s.row_lanes = s.threads / s.words;
+                const int half = (s.row_lanes + 1) / 2;
+                s.parts = shares(half, s.threads / s.width);
+                s.shared = tensors * data + sizeof(float2) * ((size_t)half * s.width + s.groups + (tensors == 1 ? 0 : 2 * s.width)) +
+                           sizeof(float) * (size_t)(tensors == 1 ? 3 : 4) * s.width;
+                if (s.shared > kMostShared) continue;
+                const double time = resident_time(p, s, V, esize, tensors);
+                if (time < least) {
+                    least = time;
+                    *best = s;
+                    found = true;
+                }
             }
         }
     }
-    return least < 1e300;
+    return found;
 }
 
-// The search takes about two microseconds; the last shapes of a thread are looked up instead.
+// The search takes some ten microseconds; the last shapes of a thread are looked up instead.
 bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     struct Entry {
         long long S, C;
@@ -1131,6 +1277,27 @@ bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     e.fits = search_resident(p, V, esize, tensors, &e.slab);
     *best = e.slab;
     return e.fits;
+}
+
+// Elements of a word: 16 bytes where addresses and rows allow them.  Rows of another length are folded, 2, 4 or 8 pixels to a
+// row, where that makes them whole words and divides the sample; otherwise words have 4 bytes or one element.
+int word_elements(Norm& p, int dtype, uint64_t addresses) {
+    const int e = sa_element_size(dtype);
+    const int a = sa_common_alignment(addresses | (uint64_t)p.C * (uint64_t)e);
+    if (a == 16) return 16 / e;
+    if (sa_common_alignment(addresses) == 16) {
+        for (int k = 2; k <= 8; k *= 2) {
+            if ((uint64_t)p.C * k * e % 16 || p.S % k || (uint64_t)p.C * k * e > 16ull * kThreads) continue;
+            Slab s;
+            const int V = a >= 4 ? 4 / e : 1;
+            if (plan_resident(p, V, e, 1, &s)) break; // short: better off in shared memory
+            p.fold = k;
+            p.S /= k;
+            p.C *= k;
+            return 16 / e;
+        }
+    }
+    return a >= 4 ? 4 / e : 1;
 }
 
 // Lets a kernel have more than 48 KiB of dynamic shared memory, once for each kernel and device.
@@ -1190,7 +1357,7 @@ size_t ring_bytes(size_t tile) {
 template <class T, int V>
 cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream) {
     Slab s;
-    if (plan_resident(p, V, sizeof(T), 1, &s))
+    if (p.fold == 1 && plan_resident(p, V, sizeof(T), 1, &s))
         return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, (T*)out, (const T*)x, mean, rstd, s);
     s = cut(p, V);
     const size_t params = sizeof(float) * 3 * (size_t)s.width;
@@ -1208,31 +1375,33 @@ template <class T, int V>
 cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const float* mean, const float* rstd,
                      Norm p, void* workspace, cudaStream_t stream) {
     Slab s;
-    if (plan_resident(p, V, sizeof(T), 2, &s)) {
+    if (p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s)) {
         float2* const sums = p.N > 1 && (dweight || dbias) ? (float2*)workspace : nullptr;
         const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
         if (e != cudaSuccess || !sums) return e;
-        return launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, false, stream, sums, dweight,
+        return launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
                       dbias, p);
     }
     s = cut(p, V);
     const unsigned grid = (unsigned)((long long)p.N * s.slabs * s.blocks);
     const size_t params = sizeof(float) * 5 * (size_t)s.width;
     s.shared = ring_bytes<T, V>(s.shared); // streams, then tile; the parameters behind
-    float2* const partial = (float2*)workspace;
+    float2* const partial = (float2*)workspace; // [N][runs][C]
     float2* const sums = partial + (long long)p.N * s.blocks * p.C;
-    float2* const means = sums + (long long)p.N * p.C;
+    const long long channels = p.C / p.fold;
     cudaError_t e = launch(sa_norm_backward_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)dout,
                            (const T*)x, mean, rstd, partial, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_backward_join_kernel, (unsigned)(p.N * p.G), kThreads, 0, true, stream, partial, rstd, sums, means, s);
+        e = launch(sa_norm_backward_sums_kernel, (unsigned)(p.N * ((channels + 31) / 32)), 1024, 0, true, stream, partial, rstd, sums, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)dx, (const T*)dout, (const T*)x, mean,
-                   rstd, means, s);
-    if (e == cudaSuccess && (dweight || dbias))
-        e = launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
+        e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)dx, (const T*)dout, (const T*)x,
+                   mean, rstd, sums, s);
+    if (e == cudaSuccess && (dweight || dbias)) {
+        p.C = channels;
+        e = launch(sa_norm_backward_params_kernel, (unsigned)((channels + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
                    dbias, p);
+    }
     return e;
 }
 
@@ -1254,28 +1423,33 @@ cudaError_t by_type(const sideaware_group_norm_t& sh, int V, F&& f) {
 
 } // namespace
 
-// Enough for words of any width, so that it follows from the shape alone.  Long samples: the partial results of all runs,
-// backward also the sums of every (n, c) and the means of every (n, g).  Resident ones: those sums, if there is more than one sample.
+// Enough for words of any width, so that it follows from the shape alone.  Streamed samples: the partial results of all runs,
+// backward also the sums of every (n, c).  Resident ones: those sums, if there is more than one sample.
 size_t sa_group_norm_workspace(const sideaware_group_norm_t& sh, bool backward) {
     const int e = sa_element_size(sh.dtype);
     long long most = 0;
+    auto streamed = [&](const Norm& p, int V) {
+        const Slab s = cut(p, V);
+        return backward ? (long long)p.N * s.blocks * p.C + (long long)sh.N * sh.C : (long long)p.N * s.blocks * s.slabs * s.groups;
+    };
     for (int V : {16 / e, 4 / e, 1}) {
         if (sh.C % V) continue;
-        Norm p = describe(sh, nullptr, nullptr);
+        const Norm p = describe(sh, nullptr, nullptr);
         Slab s;
-        long long entries = backward && sh.N > 1 ? (long long)sh.N * sh.C : 0;
-        if (!plan_resident(p, V, e, backward ? 2 : 1, &s)) {
-            entries = (long long)sh.N * cut(p, V).blocks * sh.C + (backward ? (long long)sh.N * (sh.C + sh.G) : 0);
-        }
+        const long long entries = plan_resident(p, V, e, backward ? 2 : 1, &s) ? (backward && sh.N > 1 ? (long long)sh.N * sh.C : 0) : streamed(p, V);
         if (entries > most) most = entries;
     }
+    Norm p = describe(sh, nullptr, nullptr);
+    const int V = word_elements(p, sh.dtype, 0);
+    if (p.fold > 1 && streamed(p, V) > most) most = streamed(p, V);
     return (size_t)most * sizeof(float2);
 }
 
 cudaError_t sa_launch_group_norm(void* out, float* mean, float* rstd, const void* x, const void* weight, const void* bias,
                                  const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream) {
-    const Norm p = describe(sh, weight, bias);
-    return by_type(sh, word_elements(sh, (uint64_t)out | (uint64_t)x), [&](auto type, auto v) {
+    Norm p = describe(sh, weight, bias);
+    const int V = word_elements(p, sh.dtype, (uint64_t)out | (uint64_t)x);
+    return by_type(sh, V, [&](auto type, auto v) {
         return forward<decltype(type), v.value>(out, mean, rstd, x, p, workspace, stream);
     });
 }
@@ -1283,8 +1457,9 @@ cudaError_t sa_launch_group_norm(void* out, float* mean, float* rstd, const void
 cudaError_t sa_launch_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const float* mean,
                                           const float* rstd, const void* weight, const void* bias,
                                           const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream) {
-    const Norm p = describe(sh, weight, bias);
-    return by_type(sh, word_elements(sh, (uint64_t)dx | (uint64_t)dout | (uint64_t)x), [&](auto type, auto v) {
+    Norm p = describe(sh, weight, bias);
+    const int V = word_elements(p, sh.dtype, (uint64_t)dx | (uint64_t)dout | (uint64_t)x);
+    return by_type(sh, V, [&](auto type, auto v) {
         return backward<decltype(type), v.value>(dx, dweight, dbias, dout, x, mean, rstd, p, workspace, stream);
     });
 }

@@ -156,6 +156,9 @@ NORM_SHAPES = [  # N, S, C, G
     (1, 1, 1, 1), (2, 7, 6, 3), (1, 64, 1280, 32), (3, 33, 96, 32), (2, 1000, 320, 32), (1, 5, 2048, 1), (2, 300, 40, 40),
     (1, 4099, 48, 16), (4, 257, 64, 2), (1, 1, 512, 32), (2, 9, 30, 2), (1, 70001, 8, 4), (17, 16, 160, 32), (1, 3000, 4104, 8),
     (2, 16384, 128, 32), (1, 40000, 256, 32),
+    # long samples: whole words, rows folded to whole words (2, 4 and 8 pixels), rows that cannot be
+    (2, 150000, 24, 3), (1, 300000, 64, 4), (2, 100000, 330, 2), (1, 600000, 6, 2), (2, 262144, 1, 1), (1, 400004, 10, 1), (3, 80001, 12, 3),
+    (1, 200001, 5, 5), (1, 30000, 2056, 8),
 ]
 
 

@@ -37,37 +37,27 @@ __device__ __forceinline__ void philox(uint4 (&c)[U], uint32_t k0, uint32_t k1) 
     }
 }
 
-// Which 16-bit halves of w equal h (given twice): the classic zero-byte test on halves, non-zero if any is.
-__device__ __forceinline__ uint32_t equal_halves(uint32_t w, uint32_t hh) {
-    const uint32_t x = w ^ hh;
-    return (x - 0x00010001u) & ~x & 0x80008000u;
+// Whether one of the eight 16-bit halves of b equals `upper` (and there is a lower half to look at): the halves' differences
+// by exclusive or, their minimum two at a time, then the classic test for a zero half.
+__device__ __forceinline__ bool has_tie(const uint4& b, const Draw& d) {
+    const uint32_t twice = d.upper << 16 | d.upper;
+    uint32_t m = b.x ^ twice;
+    asm("min.u16x2 %0, %0, %1;" : "+r"(m) : "r"(b.y ^ twice));
+    asm("min.u16x2 %0, %0, %1;" : "+r"(m) : "r"(b.z ^ twice));
+    asm("min.u16x2 %0, %0, %1;" : "+r"(m) : "r"(b.w ^ twice));
+    return ((m - 0x00010001u) & ~m & 0x80008000u) != 0u && d.upper < 65536u && d.lower != 0u;
 }
 
-// Bit i: element i of group g is kept, once its upper half has tied: the lower half decides.
-__device__ __noinline__ uint32_t settle_ties(uint32_t keep, uint4 b, uint64_t g, ulonglong2 rng, uint32_t upper, uint32_t lower) {
+// bit i: element i of group g is kept, with both halves of its number
+__device__ __noinline__ uint32_t exact_mask(uint4 b, uint64_t g, ulonglong2 rng, uint32_t upper, uint32_t lower) {
     uint4 c[1] = {make_uint4((uint32_t)g, (uint32_t)(g >> 32) | 0x80000000u, (uint32_t)rng.y, (uint32_t)(rng.y >> 32))};
     philox<1>(c, (uint32_t)rng.x, (uint32_t)(rng.x >> 32));
     const uint32_t first[4] = {b.x, b.y, b.z, b.w}, second[4] = {c[0].x, c[0].y, c[0].z, c[0].w};
+    uint32_t keep = 0;
     for (int i = 0; i < 8; ++i) {
         const int shift = 16 * (i & 1);
-        if (((first[i / 2] >> shift) & 0xffffu) == upper && ((second[i / 2] >> shift) & 0xffffu) < lower) keep &= ~(1u << i);
-    }
-    return keep;
-}
-
-// bit i: element i of the group is kept
-__device__ __forceinline__ uint32_t keep_mask(const uint4& b, uint64_t g, ulonglong2 rng, const Draw& d) {
-    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-    uint32_t keep = 0, tie = 0;
-    if (d.upper < 65536u) {
-        const uint32_t top = d.upper << 16, twice = top | d.upper;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            keep |= (w[k] << 16) >= top ? 1u << (2 * k) : 0u; // the halves as the upper 16 bits of a word
-            keep |= w[k] >= top ? 2u << (2 * k) : 0u;
-            tie |= equal_halves(w[k], twice);
-        }
-        if (tie != 0u && d.lower != 0u) keep = settle_ties(keep, b, g, rng, d.upper, d.lower);
+        const uint32_t u = (first[i / 2] >> shift) & 0xffffu, v = (second[i / 2] >> shift) & 0xffffu;
+        if (u > upper || (u == upper && v >= lower)) keep |= 1u << i;
     }
     return keep;
 }
@@ -82,6 +72,25 @@ struct Eight {
         for (int k = 0; k < kWords; ++k) w[k] = sa_load_stream<T, kPer>(p + k * kPer);
     }
 };
+
+// A group's results; kept(i): element i is kept.
+template <class T, bool RESIDUAL, class F>
+__device__ __forceinline__ void finish(T* out, Eight<T>& a, const Eight<T>& r, float scale, F&& kept) {
+    const F2 both = f2(scale, scale);
+#pragma unroll
+    for (int k = 0; k < Eight<T>::kWords; ++k) {
+#pragma unroll
+        for (int j = 0; j < Eight<T>::kPer / 2; ++j) {
+            const int e = k * Eight<T>::kPer + 2 * j;
+            float p, q;
+            split(pair_of(a.w[k], j) * both, p, q);
+            F2 v = f2(kept(e) ? p : 0.0f, kept(e + 1) ? q : 0.0f);
+            if (RESIDUAL) v = v + pair_of(r.w[k], j);
+            set_pair(a.w[k], j, v);
+        }
+        sa_store_stream<T, Eight<T>::kPer>(out + k * Eight<T>::kPer, a.w[k]);
+    }
+}
 
 // U groups of each thread, kThreads groups apart.
 template <class T, bool RESIDUAL, int U>
@@ -105,27 +114,21 @@ sa_dropout_kernel(T* out, const T* x, const T* residual, const ulonglong2* rng_s
         c[u] = make_uint4((uint32_t)g, (uint32_t)(g >> 32), (uint32_t)rng.y, (uint32_t)(rng.y >> 32));
     }
     philox<U>(c, (uint32_t)rng.x, (uint32_t)(rng.x >> 32));
+    const uint32_t top = d.upper << 16; // a half against `upper`, both as the upper half of a word
+    const bool none = d.upper >= 65536u;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint64_t g = g0 + u * kThreads, i0 = g * 8;
-        if (i0 >= n) continue;
-        const uint32_t keep = keep_mask(c[u], g, rng, d);
         if (i0 + 8 <= n) {
-            const F2 scale = f2(d.scale, d.scale);
-#pragma unroll
-            for (int k = 0; k < Eight<T>::kWords; ++k) {
-#pragma unroll
-                for (int j = 0; j < Eight<T>::kPer / 2; ++j) {
-                    const int e = k * Eight<T>::kPer + 2 * j;
-                    float p, q;
-                    split(pair_of(a[u].w[k], j) * scale, p, q);
-                    F2 v = f2((keep >> e) & 1u ? p : 0.0f, (keep >> e) & 2u ? q : 0.0f);
-                    if (RESIDUAL) v = v + pair_of(r[u].w[k], j);
-                    set_pair(a[u].w[k], j, v);
-                }
-                sa_store<T, Eight<T>::kPer>(out + i0 + k * Eight<T>::kPer, a[u].w[k]);
+            if (none || has_tie(c[u], d)) {
+                const uint32_t keep = none ? 0u : exact_mask(c[u], g, rng, d.upper, d.lower);
+                finish<T, RESIDUAL>(out + i0, a[u], r[u], d.scale, [&](int i) { return (keep >> i) & 1u; });
+            } else {
+                const uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+                finish<T, RESIDUAL>(out + i0, a[u], r[u], d.scale, [&](int i) { return (i & 1 ? w[i / 2] : w[i / 2] << 16) >= top; });
             }
-        } else { // the last, partial group
+        } else if (i0 < n) { // the last, partial group
+            const uint32_t keep = none ? 0u : exact_mask(c[u], g, rng, d.upper, d.lower);
             for (int j = 0; j < 8 && i0 + j < n; ++j) {
                 float v = (keep >> j) & 1u ? sa_to_float(x[i0 + j]) * d.scale : 0.0f;
                 if (RESIDUAL) v += sa_to_float(residual[i0 + j]);
@@ -144,7 +147,7 @@ sa_dropout_unaligned_kernel(T* out, const T* x, const T* residual, const ulonglo
     const ulonglong2 rng = __ldg(rng_state);
     uint4 c[1] = {make_uint4((uint32_t)g, (uint32_t)(g >> 32), (uint32_t)rng.y, (uint32_t)(rng.y >> 32))};
     philox<1>(c, (uint32_t)rng.x, (uint32_t)(rng.x >> 32));
-    const uint32_t keep = keep_mask(c[0], g, rng, d);
+    const uint32_t keep = d.upper >= 65536u ? 0u : exact_mask(c[0], g, rng, d.upper, d.lower);
     for (int j = 0; j < 8 && i0 + j < n; ++j) {
         float v = (keep >> j) & 1u ? sa_to_float(x[i0 + j]) * d.scale : 0.0f;
         if (RESIDUAL) v += sa_to_float(residual[i0 + j]);
@@ -156,8 +159,9 @@ template <class T>
 cudaError_t launch(void* out, const void* x, const void* residual, const void* rng, const Draw& d, size_t n, cudaStream_t stream) {
     const bool aligned = sa_common_alignment((uint64_t)out | (uint64_t)x | (uint64_t)residual) == 16;
     const uint64_t groups = (n + 7) / 8;
-    // four groups of a thread (two of fp32: 64 bytes of x in flight either way) once that leaves every SM its threads
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;
+    // two groups of a thread share the key schedule once that leaves every SM its threads (four: 5 % slower, the registers cost
+    // warps); fp32 moves twice the bytes for the same numbers and is 3 % faster with one
+    constexpr int U = sizeof(T) == 2 ? 2 : 1;
     const int each = !aligned || groups < 148ull * 2048 * U ? 1 : U;
     const uint64_t blocks = (groups + (uint64_t)kThreads * each - 1) / ((uint64_t)kThreads * each);
     if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;

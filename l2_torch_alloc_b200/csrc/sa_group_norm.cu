@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxCluster = 8;                                          // blocks of a cluster that every GPU schedules
-constexpr int kResidentThreads = 512;                                   // threads of a resident block, at most
+constexpr int kResidentThreads = 1024;                                  // threads of a resident block, at most
 constexpr int kResidentRegisters = 64, kResidentBackwardRegisters = 80; // 32 and 25 warps on an SM
 
 struct Norm {
@@ -1177,8 +1177,8 @@ Norm describe(const sideaware_group_norm_t& sh, const void* weight, const void* 
 constexpr int kMostShared = 226 * 1024; // dynamic shared memory of a block
 
 // How a resident launch would run, in microseconds.  The form is a sum of what an SM has to do in each round of blocks; the
-// constants were fitted to 2,600 measured launches (26 shapes, forward and backward, all slab widths, cluster sizes and block
-// sizes) with a mean error of 14 %: the choice that follows from it took 4 % longer than each shape's best one.
+// constants were fitted to 3,000 measured launches (13 shapes, forward and backward, all slab widths, cluster sizes and block
+// sizes) with a mean error of 13 %: the choice that follows from it took 5 % longer than each shape's best one.
 double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors) {
     // blocks that run at once when each has an SM (or a share of one) to itself: a cluster stays inside a GPC, so sizes that
     // do not divide a GPC's SMs leave some idle (cudaOccupancyMaxActiveClusters)
@@ -1194,25 +1194,26 @@ double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors
     const double segment = (double)s.width * esize, bytes = (double)s.rows * s.words * V * esize;
     double ragged = (s.width * esize) % 32 ? (segment + 16.0) / segment : 1.0;
     if (segment < 64.0) ragged *= 2.0 - segment / 64.0;
-    const double memory = of_sm * bytes * (tensors + 1) * ragged / 43e3;
-    // arithmetic: cycles of a warp for a row of its words (V = 8), on four schedulers, fewer than 18 warps do not fill them
-    const double warps = of_sm * s.threads / 32, row = (tensors == 1 ? 34.0 : 214.0) * std::max(V / 8.0, 0.3) * (esize == 4 ? 1.3 : 1.0);
+    const double memory = of_sm * bytes * (tensors + 1) * ragged / 59e3;
+    // arithmetic: cycles of a warp for a row of its words (V = 8), on four schedulers, fewer than 20 warps do not fill them
+    const double warps = of_sm * s.threads / 32, row = (tensors == 1 ? 54.0 : 237.0) * std::max(V / 8.0, 0.3) * (esize == 4 ? 1.3 : 1.0);
     const double lanes = std::ceil((double)s.rows / s.row_lanes);
-    const double arithmetic = of_sm * lanes * (s.threads / 32) * row / 4 / 1900 / std::min(1.0, warps / 18.0);
-    const double fixed = 3.0 + (s.blocks > 1 ? 1.0 : 0.0) + 0.4 * s.blocks + (tensors == 1 ? 0.0 : 0.7); // latencies and barriers
-    return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 5.5;
+    const double arithmetic = of_sm * lanes * (s.threads / 32) * row / 4 / 1900 / std::min(1.0, warps / 20.0);
+    const double fixed = 3.8 + (s.blocks > 1 ? 1.4 : 0.0) + 0.26 * s.blocks + (tensors == 1 ? 0.0 : 0.7); // latencies and barriers
+    return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 6.0;
 }
 
 // The same for the way of long samples: three or four launches (fitted to 0.2-134 MB of x; within 20 %).
 double streamed_time(const Norm& p, int V, int esize, int tensors) {
     const double mb = (double)p.N * (double)p.S * (double)p.C * esize * 1e-6 * (V * esize == 16 ? 1.0 : V * esize == 4 ? 4.0 : 8.0);
-    return tensors == 1 ? 14.6 + 0.48 * mb : 28.0 + 0.75 * mb;
+    return tensors == 1 ? 17.0 + 0.45 * mb : 31.0 + 0.75 * mb;
 }
 
 // Whether the groups of a sample are to be resident, and how: every slab width (multiples of the narrowest one that is whole
 // words, up to 512 bytes of a row), cluster size and block size that fits, against each other and against streaming.
 bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     if (p.S > 1 << 20) return false;
+    const int registers = tensors == 1 ? kResidentRegisters : kResidentBackwardRegisters;
     int unit = 1; // groups of the narrowest slab
     while ((unit * (long long)p.D) % V) ++unit;
     double least = streamed_time(p, V, esize, tensors);
@@ -1220,7 +1221,7 @@ bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     for (int m = 1; m == 1 || unit * (m - 1) < p.G; ++m) {
         const int groups = unit * m < p.G ? unit * m : p.G;
         const long long width = (long long)groups * p.D;
-        if (width % V || width / V > kResidentThreads / 2 || (m > 1 && width * esize > 512)) break;
+        if (width % V || width / V > 256 || (m > 1 && width * esize > 512)) break;
         Slab s{};
         s.p = p;
         s.groups = groups;
@@ -1235,7 +1236,7 @@ bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
             if ((s.blocks > 1 && s.rows < 8) || (double)p.N * s.slabs * s.blocks > 1e9) break;
             const size_t data = ((size_t)s.rows * s.words * V * esize + 15) / 16 * 16;
             for (s.threads = 128; s.threads <= kResidentThreads; s.threads += 128) {
-                if (s.threads < 2 * s.words) continue;
+                if (s.threads < 2 * s.words || s.threads * registers > 65536) continue;
                 s.row_lanes = s.threads / s.words;
                 const int half = (s.row_lanes + 1) / 2;
                 s.parts = shares(half, s.threads / s.width);

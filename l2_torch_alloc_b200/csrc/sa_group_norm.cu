@@ -6,23 +6,31 @@
 //   dbias = sum_n A, dweight = sum_n B,
 //   dx = rstd (w dz - m1 - u m2), m1 = sum_{c in g} w A / (S D), m2 = sum_{c in g} w B / (S D)
 //
-// Statistics: a thread takes the exact two-step mean and squared deviation of a few rows at a time and joins them with
-// the pairwise update of Chan, Golub and LeVeque (1983), all in fp32: no cancellation however far the mean is from zero.
-// All sums go through fixed trees (no atomics): the same inputs give the same bits.
+// Statistics: sums about a value that is one of the data, kept for a few rows, then joined with the pairwise update of Chan,
+// Golub and LeVeque (1983), all in fp32: no cancellation however far the mean is from zero.  All sums go through fixed trees
+// (no atomics): the same inputs give the same bits.
 //
-// Two ways, chosen by plan_resident below:
+// Two ways, chosen by search_resident below:
 //  * resident: a thread-block cluster owns some neighbouring groups of one sample, all rows of them lie in the shared
 //    memory of its blocks, which exchange their statistics through distributed shared memory.  One launch, each element
 //    is read once and written once.
-//  * for samples too long for that, three launches: partial statistics of runs of rows, joining them, applying them.
+//  * streamed, for samples too long for that: partial statistics of runs of rows, joining them, applying them; three
+//    launches that overlap, x is read twice (a part of it from L2).
+//
+// Bound and measured on a B200 (device time of a call, three sets of inputs in turn):
+//  * resident: the phases of a block follow one another, and each moves about 4 TB/s alone.  8 x 4096 x 320 bf16: 16.7 us (6.4
+//    at the copy's rate), of 31,000 cycles 12,000 are for the rows to arrive, 5,000 for the statistics to go around and
+//    11,500 for SiLU and the stores (without SiLU: 1.4 us less).  Backward the activation's derivative is worked out twice, 24
+//    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.2 us.
+//  * streamed: HBM.  2 x 262144 x 128 bf16: 74.5 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
+//    us for the copy-like second pass.
+//  * small: latency.  1 x 64 x 1280 bf16: 5 us, of which 0.9 is the HBM's latency and 1.5 the joining of statistics.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <cmath>
 #include <mutex>
-#include <set>
 #include <type_traits>
-#include <utility>
 
 #include "sa_elem.cuh"
 #include "sa_kernels.hpp"
@@ -33,8 +41,8 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxCluster = 8;                                          // blocks of a cluster that every GPU schedules
-constexpr int kResidentThreads = 1024;                                  // threads of a resident block, at most
+constexpr int kMaxCluster = 8; // blocks of a cluster that every GPU schedules
+constexpr int kResidentThreads = 1024; // threads of a resident block, at most
 constexpr int kResidentRegisters = 64, kResidentBackwardRegisters = 80; // 32 and 25 warps on an SM
 
 struct Norm {
@@ -74,7 +82,7 @@ __device__ __forceinline__ float sigmoid(float z) {
 // ---------------------------------------------------------------------------
 struct Slab {
     Norm p;
-    int groups, width;     // channels of a slab, a whole number of words; resident: whole groups, so many
+    int groups, width;     // groups of a slab (streamed: that it touches, at most), its channels: a whole number of words
     int words;             // words of a row
     int row_lanes;         // rows a block takes at a time: a thread has one word of every row_lanes-th row
     int slabs;             // of a sample
@@ -117,8 +125,8 @@ __device__ __forceinline__ Place place_of(const Slab& s, uint32_t block) {
 }
 
 // This thread's words of its block's rows from global into shared memory, without passing through registers (words of 4
-// bytes or more); complete for this thread after wait_for_rows.  The rows come in kStages groups, so that the first ones can
-// be worked on while the others travel.
+// bytes or more).  The rows come in kStages groups, so that the first ones can be worked on while the others travel; a thread
+// waits for its own words only.  (Through registers instead: 8 to 40 % slower; hints to fetch whole lines: no difference.)
 constexpr int kStages = 4;
 __device__ __forceinline__ int stage_end(int rows, int stage) { return stage == kStages - 1 ? rows : rows * (stage + 1) / kStages; }
 
@@ -339,7 +347,7 @@ __device__ __forceinline__ float2 channel_sum(const Slab& s, const float2* tile,
 }
 
 // ---------------------------------------------------------------------------
-// samples too long for that: partial results of runs of rows, joined, then applied
+// streamed: partial results of runs of rows, joined, then applied
 // ---------------------------------------------------------------------------
 // A thread's rows (one word of each) on their way through a ring in shared memory that only this thread uses: four stages of
 // ROWS rows are in flight.  16 words of each thread in all (64 KiB of a block, three blocks of an SM): 4 rows of one tensor or
@@ -444,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 3)
 sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     extern __shared__ __align__(16) unsigned char memory[];
-    float2* const tile = (float2*)memory;                                   // [lanes][width], after the stream has passed
-    float* const centre = (float*)(memory + s.shared); // [width] the means of row lane 0
+    float2* const tile = (float2*)memory;              // [lanes][width], after the stream has passed
+    float* const centre = (float*)(memory + s.shared); // [width] each: the means of row lane 0, then the channels'; m2
     may_follow();
     const Place w = place_of<V>(s, blockIdx.x);
     const Norm& p = s.p;
@@ -614,7 +622,7 @@ sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict_
     extern __shared__ __align__(16) unsigned char memory[];
     constexpr int kRows = kRingWords / 2 / kStreamStages;
     constexpr size_t kRing = kRingWords / 2 * kThreads * sizeof(SaVec<T, V>);
-    float2* const tile = (float2*)memory;              // [lanes][width], after the streams have passed
+    float2* const tile = (float2*)memory;             // [lanes][width], after the streams have passed
     float* const slope = (float*)(memory + s.shared); // [width] each: weight * rstd, bias, mean
     float* const bias = slope + s.width;
     float* const centre = bias + s.width;
@@ -715,7 +723,7 @@ sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict
     if (dweight) sa_set_param(dweight, c, p.param_dtype, s.y);
 }
 
-
+// The rows are taken from the end, as above.
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, 3)
 sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -1301,26 +1309,34 @@ int word_elements(Norm& p, int dtype, uint64_t addresses) {
     return a >= 4 ? 4 / e : 1;
 }
 
-// Lets a kernel have more than 48 KiB of dynamic shared memory, once for each kernel and device.
+// Lets a kernel have more than 48 KiB of dynamic shared memory, once for each kernel and device (a full table only means that
+// the attribute is set again).
 cudaError_t allow_shared(const void* kernel, size_t bytes) {
     if (bytes <= 48 * 1024) return cudaSuccess;
+    struct Allowed {
+        const void* kernel;
+        int device;
+    };
     static std::mutex mu;
-    static std::set<std::pair<const void*, int>> allowed;
+    static Allowed allowed[256];
+    static int count = 0;
     int device = 0;
     cudaGetDevice(&device);
     std::lock_guard<std::mutex> lock(mu);
-    if (allowed.count({kernel, device})) return cudaSuccess;
+    for (int i = 0; i < count; ++i)
+        if (allowed[i].kernel == kernel && allowed[i].device == device) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
-    if (e == cudaSuccess) allowed.insert({kernel, device});
+    if (e == cudaSuccess && count < 256) allowed[count++] = Allowed{kernel, device};
     return e;
 }
 
 // `follows`: the launch may begin while the previous kernel of the same call ends
 template <class... P, class... Args>
-cudaError_t launch(void (*kernel)(P...), unsigned grid, int threads, size_t shared, bool follows, cudaStream_t stream, Args... args) {
+cudaError_t launch(void (*kernel)(P...), long long grid, int threads, size_t shared, bool follows, cudaStream_t stream, Args... args) {
     if (const cudaError_t e = allow_shared((const void*)kernel, shared); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
+    if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
@@ -1364,9 +1380,9 @@ cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, 
     const size_t params = sizeof(float) * 3 * (size_t)s.width;
     s.shared = ring_bytes<T, V>(s.shared); // stream, then tile; the parameters behind
     float2* const partial = (float2*)workspace;
-    const unsigned grid = (unsigned)((long long)p.N * s.slabs * s.blocks);
+    const long long grid = (long long)p.N * s.slabs * s.blocks;
     cudaError_t e = launch(sa_norm_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)x, partial, s);
-    if (e == cudaSuccess) e = launch(sa_norm_join_kernel, (unsigned)(p.N * p.G), kThreads, 0, true, stream, partial, mean, rstd, s);
+    if (e == cudaSuccess) e = launch(sa_norm_join_kernel, (long long)p.N * p.G, kThreads, 0, true, stream, partial, mean, rstd, s);
     if (e == cudaSuccess)
         e = launch(sa_norm_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)out, (const T*)x, mean, rstd, s);
     return e;
@@ -1381,11 +1397,11 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
         const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
         if (e != cudaSuccess || !sums) return e;
-        return launch(sa_norm_backward_params_kernel, (unsigned)((p.C + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
+        return launch(sa_norm_backward_params_kernel, (p.C + kThreads - 1) / kThreads, kThreads, 0, true, stream, sums, dweight,
                       dbias, p);
     }
     s = cut(p, V);
-    const unsigned grid = (unsigned)((long long)p.N * s.slabs * s.blocks);
+    const long long grid = (long long)p.N * s.slabs * s.blocks;
     const size_t params = sizeof(float) * 5 * (size_t)s.width;
     s.shared = ring_bytes<T, V>(s.shared); // streams, then tile; the parameters behind
     float2* const partial = (float2*)workspace; // [N][runs][C]
@@ -1394,13 +1410,13 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     cudaError_t e = launch(sa_norm_backward_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)dout,
                            (const T*)x, mean, rstd, partial, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_backward_sums_kernel, (unsigned)(p.N * ((channels + 31) / 32)), 1024, 0, true, stream, partial, rstd, sums, s);
+        e = launch(sa_norm_backward_sums_kernel, p.N * ((channels + 31) / 32), 1024, 0, true, stream, partial, rstd, sums, s);
     if (e == cudaSuccess)
         e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)dx, (const T*)dout, (const T*)x,
                    mean, rstd, sums, s);
     if (e == cudaSuccess && (dweight || dbias)) {
         p.C = channels;
-        e = launch(sa_norm_backward_params_kernel, (unsigned)((channels + kThreads - 1) / kThreads), kThreads, 0, true, stream, sums, dweight,
+        e = launch(sa_norm_backward_params_kernel, (channels + kThreads - 1) / kThreads, kThreads, 0, true, stream, sums, dweight,
                    dbias, p);
     }
     return e;

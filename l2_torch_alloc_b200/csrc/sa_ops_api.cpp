@@ -26,13 +26,22 @@ cudaError_t refuse(const char* what, const char* why) {
     return cudaErrorInvalidValue;
 }
 
-// runs `launch` on the device's context and records what went wrong
+// Runs `launch` on the device and records what went wrong.  These kernels need nothing of the library's per-device set-up
+// (topology, counters), so a first call may be part of a stream capture; launches are counted once that set-up exists.
 template <class F>
 cudaError_t on_device(const char* what, int device, int launches, F&& launch) {
-    SaDevice* dev = sa_device(device);
-    if (!dev) return cudaErrorInitializationError;
-    SaScopedDevice guard(dev->id);
-    dev->launches.fetch_add((unsigned long long)launches);
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count <= 0 || (device < 0 && cudaGetDevice(&device) != cudaSuccess)) {
+        cudaGetLastError();
+        sa_set_error("%s: no CUDA device available (this library has no CPU path)", what);
+        return cudaErrorInitializationError;
+    }
+    if (device >= count) {
+        sa_set_error("%s: device %d out of range (%d devices)", what, device, count);
+        return cudaErrorInvalidDevice;
+    }
+    SaScopedDevice guard(device);
+    if (SaDevice* dev = sa_device_if_ready(device)) dev->launches.fetch_add((unsigned long long)launches);
     const cudaError_t e = launch();
     if (e != cudaSuccess) sa_set_error("%s launch: %s", what, cudaGetErrorString(e));
     return e;

@@ -143,9 +143,9 @@ def philox(counter, key):
     return c
 
 
-def keep_mask(n, seed, call, p):
-    """Which of n elements are kept, in numpy (uint64)."""
-    group = np.arange((n + 7) // 8, dtype=np.uint64)
+def keep_mask(n, seed, call, p, first=0):
+    """Which of n elements from element `first` on (a multiple of 8) are kept, in numpy (uint64)."""
+    group = np.arange(first // 8, first // 8 + (n + 7) // 8, dtype=np.uint64)
     lo, mask = np.uint64(32), np.uint64(0xFFFFFFFF)
 
     def blocks(second):

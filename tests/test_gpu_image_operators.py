@@ -106,6 +106,21 @@ def test_rope_axes_strides(sa, layout):
             assert torch.equal(whole, x._base if x._base is not None else x), "nothing outside the view was written"
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "halves"])
+def test_rope_axes_offsets_past_31_bits(sa, layout):
+    """More than 2^31 elements: the last tokens against the oracle, a middle one untouched by its neighbours' turns."""
+    T, q, kv, head = 360_000, 40, 4, 128
+    x = torch.zeros(1, T, q + 2 * kv, head, dtype=BF16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[:, -50:] = randn(1, 50, q + 2 * kv, head, seed=3, dtype=BF16)
+    before = x[:, -50:].clone()
+    positions = torch.arange(T, device="cuda").expand(2, 1, T)
+    sa.rope_axes_forward(x, positions, sa.rope_axes_spectrum((32, 32)), q, kv, layout)
+    want, bound = ref.rope(before.double(), positions[:, :, -50:], (32, 32), 10000.0, "own", q, kv, layout)
+    close(x[:, -50:], want, bound)
+    assert not x[:, :-50].any()
+
+
 def test_rope_axes_text_positions_equal_one_axis(sa):
     """Equal positions on all axes with the shared spectrum are the ordinary rotary embedding: the same as one axis, bit for bit."""
     q, kv, head = 4, 2, 64
@@ -382,6 +397,16 @@ def test_dropout_mask_bit_for_bit(sa):
         sa.dropout_forward(out, x, pair(s, c), p)
         both = float(((out != 0) & keep).double().mean())
         assert abs(both - 0.49) < 5 * (0.49 * 0.51 / n) ** 0.5
+
+
+def test_dropout_offsets_past_32_bits(sa):
+    """More than 2^32 elements: the last ones' mask, and a tail that is no whole group."""
+    n, p, rng = 2 ** 32 + 4099, 0.3, pair(11, 12)
+    x = torch.ones(n, dtype=BF16, device="cuda")
+    sa.dropout_forward(x, x, rng, p)
+    first = 2 ** 32 - 4096
+    keep = torch.from_numpy(ref.keep_mask(n - first, 11, 12, p, first)).cuda()
+    assert torch.equal(x[first:] != 0, keep)
 
 
 def test_dropout_drops_whatever_stands_there_and_works_in_place(sa):

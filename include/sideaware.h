@@ -152,11 +152,12 @@ sideaware_status_t sideaware_silu_mul_bf16(void* out, const void* a, const void*
 /* ---- operators of image and video models (no counterpart in the reference) ----
  * Element types: 0 = fp32, 1 = bf16, 2 = fp16; arithmetic in fp32, one rounding at the end.  Plain launches on
  * `stream`: nothing is kept from one call for the next, so calls may run at the same time on several streams and
- * be recorded in CUDA graphs, as long as their outputs and workspaces are their own. */
+ * be recorded in CUDA graphs (a first call too), as long as their outputs and workspaces are their own. */
 
 /* Rotary positions with several axes (time, height, width, ...), in place on packed [B, T, Nq + 2*Nkv, HS]: pair i of
  * every Q and K head is turned by pos[axis(i)][b][t] * f(i).  V heads and the elements of a head behind the first
- * 2*pairs are not touched.  Positions may be negative and need no table; the angle is exact however far they are. */
+ * 2*pairs are not touched.  Positions may be negative and need no table; f(i) / 2 pi is held to 2^-62 of a turn, so the angle is off by
+ * at most (|pos| * 2^-62 + 2^-32) turns.  The positions have as many axes as the spectrum was made with. */
 #define SIDEAWARE_ROPE_MAX_AXES 8
 #define SIDEAWARE_ROPE_MAX_PAIRS 256
 typedef struct sideaware_rope_axes_t {

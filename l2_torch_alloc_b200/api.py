@@ -328,9 +328,9 @@ class SideAware:
     def rope_axes_forward(self, qkv, positions, spectrum, n_q_heads: int, n_kv_heads: int, layout: str = "interleaved") -> None:
         """Rotary positions with several axes, in place on packed [B, T, Nq + 2 Nkv, HS] (fp32, bf16 or fp16; any strides
         over B and T): pair i of every q and k head turns by positions[axis of i, b, t] times its frequency.
-        positions: int32 or int64 [axes, B, T], any strides and values; spectrum: rope_axes_spectrum.  A head of which the
-        spectrum's pairs fill only a part keeps its remaining elements.  layout: pair i = elements (2i, 2i + 1)
-        ("interleaved") or (i, i + pairs) ("halves")."""
+        positions: int32 or int64 [axes, B, T], any strides and values, with the spectrum's axes; spectrum:
+        rope_axes_spectrum.  A head of which the spectrum's pairs fill only a part keeps its remaining elements.  layout:
+        pair i = elements (2i, 2i + 1) ("interleaved") or (i, i + pairs) ("halves")."""
         self._rope_axes(self.lib.sideaware_rope_axes_forward, "sideaware_rope_axes_forward", qkv, positions, spectrum,
                         n_q_heads, n_kv_heads, layout)
 

@@ -1332,7 +1332,7 @@ cudaError_t allow_shared(const void* kernel, size_t bytes) {
 
 // `follows`: the launch may begin while the previous kernel of the same call ends
 template <class... P, class... Args>
-cudaError_t launch(void (*kernel)(P...), long long grid, int threads, size_t shared, bool follows, cudaStream_t stream, Args... args) {
+cudaError_t launch(void (*kernel)(P...), long long grid, int threads, size_t shared, bool follows, cudaStream_t stream, int& launched, Args... args) {
     if (const cudaError_t e = allow_shared((const void*)kernel, shared); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
@@ -1345,11 +1345,13 @@ cudaError_t launch(void (*kernel)(P...), long long grid, int threads, size_t sha
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = follows && sa_pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (e == cudaSuccess) ++launched;
+    return e;
 }
 
 template <class K, class... Args>
-cudaError_t launch_clusters(K kernel, const Slab& s, cudaStream_t stream, Args... args) {
+cudaError_t launch_clusters(K kernel, const Slab& s, cudaStream_t stream, int& launched, Args... args) {
     if (const cudaError_t e = allow_shared((const void*)kernel, s.shared); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(s.p.N * s.slabs * s.blocks));
@@ -1362,7 +1364,9 @@ cudaError_t launch_clusters(K kernel, const Slab& s, cudaStream_t stream, Args..
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = s.blocks > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e == cudaSuccess) ++launched;
+    return e;
 }
 
 template <class T, int V>
@@ -1372,32 +1376,32 @@ size_t ring_bytes(size_t tile) {
 }
 
 template <class T, int V>
-cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream) {
+cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream, int& launched) {
     Slab s;
     if (p.fold == 1 && plan_resident(p, V, sizeof(T), 1, &s))
-        return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, (T*)out, (const T*)x, mean, rstd, s);
+        return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, launched, (T*)out, (const T*)x, mean, rstd, s);
     s = cut(p, V);
     const size_t params = sizeof(float) * 3 * (size_t)s.width;
     s.shared = ring_bytes<T, V>(s.shared); // stream, then tile; the parameters behind
     float2* const partial = (float2*)workspace;
     const long long grid = (long long)p.N * s.slabs * s.blocks;
-    cudaError_t e = launch(sa_norm_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)x, partial, s);
-    if (e == cudaSuccess) e = launch(sa_norm_join_kernel, (long long)p.N * p.G, kThreads, 0, true, stream, partial, mean, rstd, s);
+    cudaError_t e = launch(sa_norm_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, launched, (const T*)x, partial, s);
+    if (e == cudaSuccess) e = launch(sa_norm_join_kernel, (long long)p.N * p.G, kThreads, 0, true, stream, launched, partial, mean, rstd, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)out, (const T*)x, mean, rstd, s);
+        e = launch(sa_norm_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, launched, (T*)out, (const T*)x, mean, rstd, s);
     return e;
 }
 
 template <class T, int V>
 cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const float* mean, const float* rstd,
-                     Norm p, void* workspace, cudaStream_t stream) {
+                     Norm p, void* workspace, cudaStream_t stream, int& launched) {
     Slab s;
     if (p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s)) {
         float2* const sums = p.N > 1 && (dweight || dbias) ? (float2*)workspace : nullptr;
-        const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, (T*)dx, (const T*)dout, (const T*)x,
+        const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, launched, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
         if (e != cudaSuccess || !sums) return e;
-        return launch(sa_norm_backward_params_kernel, (p.C + kThreads - 1) / kThreads, kThreads, 0, true, stream, sums, dweight,
+        return launch(sa_norm_backward_params_kernel, (p.C + kThreads - 1) / kThreads, kThreads, 0, true, stream, launched, sums, dweight,
                       dbias, p);
     }
     s = cut(p, V);
@@ -1407,16 +1411,16 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     float2* const partial = (float2*)workspace; // [N][runs][C]
     float2* const sums = partial + (long long)p.N * s.blocks * p.C;
     const long long channels = p.C / p.fold;
-    cudaError_t e = launch(sa_norm_backward_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, (const T*)dout,
+    cudaError_t e = launch(sa_norm_backward_partial_kernel<T, V>, grid, kThreads, s.shared + params, false, stream, launched, (const T*)dout,
                            (const T*)x, mean, rstd, partial, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_backward_sums_kernel, p.N * ((channels + 31) / 32), 1024, 0, true, stream, partial, rstd, sums, s);
+        e = launch(sa_norm_backward_sums_kernel, p.N * ((channels + 31) / 32), 1024, 0, true, stream, launched, partial, rstd, sums, s);
     if (e == cudaSuccess)
-        e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, (T*)dx, (const T*)dout, (const T*)x,
+        e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, launched, (T*)dx, (const T*)dout, (const T*)x,
                    mean, rstd, sums, s);
     if (e == cudaSuccess && (dweight || dbias)) {
         p.C = channels;
-        e = launch(sa_norm_backward_params_kernel, (channels + kThreads - 1) / kThreads, kThreads, 0, true, stream, sums, dweight,
+        e = launch(sa_norm_backward_params_kernel, (channels + kThreads - 1) / kThreads, kThreads, 0, true, stream, launched, sums, dweight,
                    dbias, p);
     }
     return e;
@@ -1463,20 +1467,20 @@ size_t sa_group_norm_workspace(const sideaware_group_norm_t& sh, bool backward) 
 }
 
 cudaError_t sa_launch_group_norm(void* out, float* mean, float* rstd, const void* x, const void* weight, const void* bias,
-                                 const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream) {
+                                 const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream, int& launched) {
     Norm p = describe(sh, weight, bias);
     const int V = word_elements(p, sh.dtype, (uint64_t)out | (uint64_t)x);
     return by_type(sh, V, [&](auto type, auto v) {
-        return forward<decltype(type), v.value>(out, mean, rstd, x, p, workspace, stream);
+        return forward<decltype(type), v.value>(out, mean, rstd, x, p, workspace, stream, launched);
     });
 }
 
 cudaError_t sa_launch_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const float* mean,
                                           const float* rstd, const void* weight, const void* bias,
-                                          const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream) {
+                                          const sideaware_group_norm_t& sh, void* workspace, cudaStream_t stream, int& launched) {
     Norm p = describe(sh, weight, bias);
     const int V = word_elements(p, sh.dtype, (uint64_t)dx | (uint64_t)dout | (uint64_t)x);
     return by_type(sh, V, [&](auto type, auto v) {
-        return backward<decltype(type), v.value>(dx, dweight, dbias, dout, x, mean, rstd, p, workspace, stream);
+        return backward<decltype(type), v.value>(dx, dweight, dbias, dout, x, mean, rstd, p, workspace, stream, launched);
     });
 }

@@ -26,10 +26,11 @@ cudaError_t refuse(const char* what, const char* why) {
     return cudaErrorInvalidValue;
 }
 
-// Runs `launch` on the device and records what went wrong.  These kernels need nothing of the library's per-device set-up
-// (topology, counters), so a first call may be part of a stream capture; launches are counted once that set-up exists.
+// Runs launch(count) on the device and records what went wrong; it adds the kernels it has launched to `count`.  These kernels
+// need nothing of the library's per-device set-up (topology, counters), so a first call may be part of a stream capture;
+// launches are counted once that set-up exists.
 template <class F>
-cudaError_t on_device(const char* what, int device, int launches, F&& launch) {
+cudaError_t on_device(const char* what, int device, F&& launch) {
     int count = 0;
     if (cudaGetDeviceCount(&count) != cudaSuccess || count <= 0 || (device < 0 && cudaGetDevice(&device) != cudaSuccess)) {
         cudaGetLastError();
@@ -41,9 +42,16 @@ cudaError_t on_device(const char* what, int device, int launches, F&& launch) {
         return cudaErrorInvalidDevice;
     }
     SaScopedDevice guard(device);
-    if (SaDevice* dev = sa_device_if_ready(device)) dev->launches.fetch_add((unsigned long long)launches);
-    const cudaError_t e = launch();
+    int launched = 0;
+    const cudaError_t e = launch(launched);
+    if (SaDevice* dev = sa_device_if_ready(device)) dev->launches.fetch_add((unsigned long long)launched);
     if (e != cudaSuccess) sa_set_error("%s launch: %s", what, cudaGetErrorString(e));
+    return e;
+}
+
+// an operator of one kernel
+cudaError_t one(cudaError_t e, int& launched) {
+    if (e == cudaSuccess) ++launched;
     return e;
 }
 
@@ -73,9 +81,9 @@ cudaError_t rope_axes(const char* what, void* qkv, const void* positions, const 
     if (row > (1ll << 30)) return refuse(what, "more than 2^30 elements of a row");
     const long long sb = sh->stride_b, st = sh->stride_t;
     if ((sh->T > 1 && (st < row || st > (1ll << 40))) || (sh->B > 1 && (sb < row || sb > (1ll << 46)))) return refuse(what, "a stride of qkv is shorter than a row (or absurdly long)");
-    if (sh->T > 1 && sh->B > 1 && sb < (sh->T - 1) * st + row && st < (sh->B - 1) * sb + row)
+    if (sh->T > 1 && sh->B > 1 && sb < (__int128)(sh->T - 1) * st + row && st < (__int128)(sh->B - 1) * sb + row)
         return refuse(what, "rows of qkv overlap");
-    return on_device(what, device, 1, [&] { return sa_launch_rope_axes(qkv, positions, spectrum, *sh, inverse, stream); });
+    return on_device(what, device, [&](int& launched) { return one(sa_launch_rope_axes(qkv, positions, spectrum, *sh, inverse, stream), launched); });
 }
 
 // ---------------------------------------------------------------------------
@@ -103,7 +111,7 @@ cudaError_t dropout(const char* what, void* out, const void* x, const void* resi
     if (!aligned_to(out, e) || !aligned_to(x, e) || !aligned_to(residual, e) || !aligned_to(rng, 16))
         return refuse(what, "a pointer is not aligned to its elements (rng: 16 bytes)");
     if (overlaps(out, x, n * e) || overlaps(out, residual, n * e)) return refuse(what, "out overlaps an input without being that input");
-    return on_device(what, device, 1, [&] { return sa_launch_dropout(out, x, residual, rng, p, n, dtype, stream); });
+    return on_device(what, device, [&](int& launched) { return one(sa_launch_dropout(out, x, residual, rng, p, n, dtype, stream), launched); });
 }
 
 } // namespace
@@ -134,7 +142,7 @@ SA_API sideaware_status_t sideaware_rope_axes_spectrum(void* spectrum, const int
         ++used[axis];
         if (arrangement == 2) axis = (axis + 1) % axes;
     }
-    return on_device(what, device, 1, [&] { return sa_launch_rope_axes_spectrum(spectrum, turns, (int)total, (cudaStream_t)stream); });
+    return on_device(what, device, [&](int& launched) { return one(sa_launch_rope_axes_spectrum(spectrum, turns, (int)total, (cudaStream_t)stream), launched); });
 }
 
 SA_API sideaware_status_t sideaware_rope_axes_forward(void* qkv, const void* positions, const void* spectrum,
@@ -170,7 +178,9 @@ SA_API sideaware_status_t sideaware_group_norm_forward(void* out, float* mean, f
     const size_t need = sa_group_norm_workspace(*shape, false);
     if (need && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
         return refuse(what, "the workspace is missing, smaller than sideaware_group_norm_workspace says or not 16-byte aligned");
-    return on_device(what, device, 3, [&] { return sa_launch_group_norm(out, mean, rstd, x, weight, bias, *shape, workspace, (cudaStream_t)stream); });
+    return on_device(what, device, [&](int& launched) {
+        return sa_launch_group_norm(out, mean, rstd, x, weight, bias, *shape, workspace, (cudaStream_t)stream, launched);
+    });
 }
 
 SA_API sideaware_status_t sideaware_group_norm_backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x,
@@ -190,8 +200,8 @@ SA_API sideaware_status_t sideaware_group_norm_backward(void* dx, void* dweight,
     const size_t need = sa_group_norm_workspace(*shape, true);
     if (need && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
         return refuse(what, "the workspace is missing, smaller than sideaware_group_norm_workspace says or not 16-byte aligned");
-    return on_device(what, device, 4, [&] {
-        return sa_launch_group_norm_backward(dx, dweight, dbias, dout, x, mean, rstd, weight, bias, *shape, workspace, (cudaStream_t)stream);
+    return on_device(what, device, [&](int& launched) {
+        return sa_launch_group_norm_backward(dx, dweight, dbias, dout, x, mean, rstd, weight, bias, *shape, workspace, (cudaStream_t)stream, launched);
     });
 }
 

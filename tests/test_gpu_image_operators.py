@@ -734,3 +734,24 @@ class Definition(torch.autograd.Function):
     def backward(ctx, d):
         positions, pairs, q, kv = ctx.rest
         return ref.rope(d, positions, pairs, 100.0, "own", q, kv, "halves", inverse=True)[0], None, None, None, None
+
+
+def test_launches_are_counted_as_they_are_made(sa):
+    """Two samples: the resident form has one kernel forward, two backward; the streamed one three and four."""
+
+    def count(call):
+        before = sa.stats()["kernel_launches"]
+        call()
+        return sa.stats()["kernel_launches"] - before
+
+    x = randn(1, 4, 6, 16, seed=1)
+    spectrum = sa.rope_axes_spectrum((4,))
+    positions = torch.zeros(1, 1, 4, dtype=torch.int32, device="cuda")
+    assert count(lambda: sa.rope_axes_forward(x, positions, spectrum, 2, 2)) == 1
+    assert count(lambda: sa.dropout_forward(torch.empty_like(x), x, pair(1, 2), 0.5)) == 1
+    for rows, forward, backward in ((64, 1, 2), (300000, 3, 4)):
+        x = randn(2, rows, 64, seed=2, dtype=BF16)
+        w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+        mean, rstd = torch.empty(2, 8, device="cuda"), torch.empty(2, 8, device="cuda")
+        assert count(lambda: sa.group_norm_forward(torch.empty_like(x), mean, rstd, x, w, b, 8)) == forward
+        assert count(lambda: sa.group_norm_backward(torch.empty_like(x), torch.empty_like(w), torch.empty_like(b), x, x, mean, rstd, w, b, 8)) == backward

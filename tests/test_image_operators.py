@@ -41,6 +41,12 @@ def test_rope_axes_refuses(sa, name, change, text):
     refused(sa, getattr(sa.lib, name)(P, P, P, ctypes.byref(rope_shape(**change)), 0, None), text)
 
 
+def test_rope_axes_overlap_is_found_past_64_bits(sa):
+    """(T - 1) * stride_t is 2^64 - 2^40 here: rows of the second sample lie among those of the first."""
+    s = rope_shape(B=2, T=1 << 24, stride_t=1 << 40, stride_b=1 << 41)
+    refused(sa, sa.lib.sideaware_rope_axes_forward(P, P, P, ctypes.byref(s), 0, None), "overlap")
+
+
 def test_rope_axes_refuses_pointers(sa):
     call, s = sa.lib.sideaware_rope_axes_forward, rope_shape()
     for args in ((None, P, P), (P, None, P), (P, P, None)):

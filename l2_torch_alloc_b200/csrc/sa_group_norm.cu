@@ -675,15 +675,24 @@ sa_norm_backward_partial_kernel(const T* __restrict__ dout, const T* __restrict_
         partial[((long long)w.n * s.blocks + w.rank) * p.C + w.first + j] = channel_sum<V>(s, tile, j);
 }
 
+// 32 channels of a block of 1024 threads, which have added up a 32nd of something each (lane = channel, warp = share): the
+// sums of channel w in warp w.
+__device__ __forceinline__ float2 joined_shares(float2 t) {
+    __shared__ float2 tile[32][33];
+    tile[threadIdx.x / 32][threadIdx.x % 32] = t;
+    __syncthreads();
+    t = tile[threadIdx.x % 32][threadIdx.x / 32];
+    return make_float2(warp_sum(t.x), warp_sum(t.y));
+}
+
 // sums[n][c] = (sum dz, sum dz u): a block for 32 channels of a sample, 32 shares of the runs
 __global__ void __launch_bounds__(1024)
 sa_norm_backward_sums_kernel(const float2* __restrict__ partial, const float* __restrict__ rstd, float2* __restrict__ sums, const __grid_constant__ Slab s) {
-    __shared__ float2 tile[32][33];
     may_follow();
     const Norm& p = s.p;
     const long long channels = p.C / p.fold;
     const uint32_t tiles = (uint32_t)((channels + 31) / 32), n = blockIdx.x / tiles;
-    const long long c = (long long)(blockIdx.x - n * tiles) * 32 + threadIdx.x % 32;
+    const long long first = (long long)(blockIdx.x - n * tiles) * 32, c = first + threadIdx.x % 32;
     const int share = threadIdx.x / 32;
     float2 t = make_float2(0.0f, 0.0f);
     await_previous();
@@ -698,29 +707,31 @@ sa_norm_backward_sums_kernel(const float2* __restrict__ partial, const float* __
             }
         }
     }
-    tile[share][threadIdx.x % 32] = t;
-    __syncthreads();
-    // warp w adds up channel w of the 32
-    t = tile[threadIdx.x % 32][share];
-    t = make_float2(warp_sum(t.x), warp_sum(t.y));
-    const long long mine = (long long)(blockIdx.x - n * tiles) * 32 + share;
+    t = joined_shares(t);
+    const long long mine = first + share;
     if (threadIdx.x % 32 == 0 && mine < channels)
         sums[(long long)n * channels + mine] = make_float2(t.x, t.y * rstd[(long long)n * p.G + (uint32_t)mine / (uint32_t)p.D]);
 }
 
-__global__ void __launch_bounds__(kThreads)
-sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict__ dweight, void* __restrict__ dbias, const __grid_constant__ Norm p) {
+// dbias, dweight = the sums of the `count` rows of sums[count][C]: a block for 32 channels, 32 shares of the rows
+__global__ void __launch_bounds__(1024)
+sa_norm_backward_params_kernel(const float2* __restrict__ sums, void* __restrict__ dweight, void* __restrict__ dbias, int count, int C, int dtype) {
     await_previous();
-    const long long c = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (c >= p.C) return;
-    float2 s = make_float2(0.0f, 0.0f);
-    for (int n = 0; n < p.N; ++n) {
-        const float2 e = sums[(long long)n * p.C + c];
-        s.x += e.x;
-        s.y += e.y;
+    const int first = (int)blockIdx.x * 32, c = first + (int)threadIdx.x % 32, share = threadIdx.x / 32;
+    float2 t = make_float2(0.0f, 0.0f);
+    if (c < C) {
+#pragma unroll 8
+        for (int r = share; r < count; r += 32) {
+            const float2 e = sums[(long long)r * C + c];
+            t.x += e.x;
+            t.y += e.y;
+        }
     }
-    if (dbias) sa_set_param(dbias, c, p.param_dtype, s.x);
-    if (dweight) sa_set_param(dweight, c, p.param_dtype, s.y);
+    t = joined_shares(t);
+    const int mine = first + share;
+    if (threadIdx.x % 32 != 0 || mine >= C) return;
+    if (dbias) sa_set_param(dbias, mine, dtype, t.x);
+    if (dweight) sa_set_param(dweight, mine, dtype, t.y);
 }
 
 // The rows are taken from the end, as above.
@@ -1394,15 +1405,17 @@ cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, 
 
 template <class T, int V>
 cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, const void* x, const float* mean, const float* rstd,
-                     Norm p, void* workspace, cudaStream_t stream, int& launched) {
+                     const Norm& p, void* workspace, cudaStream_t stream, int& launched) {
     Slab s;
+    auto join_params = [&](const float2* sums, int count, int C) {
+        return launch(sa_norm_backward_params_kernel, (C + 31) / 32, 1024, 0, true, stream, launched, sums, dweight, dbias, count, C, p.param_dtype);
+    };
     if (p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s)) {
         float2* const sums = p.N > 1 && (dweight || dbias) ? (float2*)workspace : nullptr;
         const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, launched, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
         if (e != cudaSuccess || !sums) return e;
-        return launch(sa_norm_backward_params_kernel, (p.C + kThreads - 1) / kThreads, kThreads, 0, true, stream, launched, sums, dweight,
-                      dbias, p);
+        return join_params(sums, p.N, (int)p.C);
     }
     s = cut(p, V);
     const long long grid = (long long)p.N * s.slabs * s.blocks;
@@ -1418,11 +1431,7 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     if (e == cudaSuccess)
         e = launch(sa_norm_backward_apply_kernel<T, V>, grid, kThreads, s.shared + params, true, stream, launched, (T*)dx, (const T*)dout, (const T*)x,
                    mean, rstd, sums, s);
-    if (e == cudaSuccess && (dweight || dbias)) {
-        p.C = channels;
-        e = launch(sa_norm_backward_params_kernel, (channels + kThreads - 1) / kThreads, kThreads, 0, true, stream, launched, sums, dweight,
-                   dbias, p);
-    }
+    if (e == cudaSuccess && (dweight || dbias)) e = join_params(sums, p.N, (int)channels);
     return e;
 }
 

@@ -90,7 +90,10 @@ struct Slab {
     int rows;              // of a block
     int parts;             // threads that share a channel's column when the block's threads are joined
     int threads;
-    Divisor by_words, by_width, by_D;
+    int samples;           // packed: whole samples of a tile, else 0
+    int tiles, lanes;      // packed: tiles of a slab; threads that work on a group of a sample
+    int pitch;             // packed: words from a row to the next in shared memory (odd: rows meet different banks)
+    Divisor by_words, by_width, by_D, by_S, by_groups;
     size_t shared;         // bytes of shared memory of a block
 };
 
@@ -1138,6 +1141,363 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
 }
 
 // ---------------------------------------------------------------------------
+// packed: short samples, several of them in a block's shared memory at a time
+// ---------------------------------------------------------------------------
+// A block goes through tiles of `samples` whole samples of its slab; the next tile travels while one is worked on.  A thread
+// has one word of the row, so parameters and their gradients stay in its registers; `lanes` neighbouring threads take the
+// statistics of a group of a sample: its mean about one of its elements, then the squared deviations from that.
+struct Pack {
+    int slab, first_tile;
+    int word, row_lane;
+    int channels, groups; // of this slab (the last one of a sample may be narrower)
+    long long first;      // first channel of the slab
+    int group0;           // first group of the slab
+    int g, rem;           // group of the thread's first channel in the slab, place in that group
+    bool busy;            // has a word
+};
+
+template <int V>
+__device__ __forceinline__ Pack pack_of(const Slab& s) {
+    Pack w;
+    w.slab = (int)(blockIdx.x / (uint32_t)s.blocks);
+    w.first_tile = (int)(blockIdx.x - (uint32_t)w.slab * s.blocks);
+    w.row_lane = (int)s.by_words.div(threadIdx.x);
+    w.word = (int)threadIdx.x - w.row_lane * s.words;
+    w.group0 = w.slab * s.groups;
+    w.first = (long long)w.slab * s.width;
+    w.groups = min(s.groups, s.p.G - w.group0);
+    w.channels = (int)min((long long)s.width, s.p.C - w.first);
+    w.g = (int)s.by_D.div((uint32_t)(w.word * V));
+    w.rem = w.word * V - w.g * s.p.D;
+    w.busy = w.row_lane < s.row_lanes && w.word * V < w.channels;
+    return w;
+}
+// Rows of a tile (they follow one another in memory, whole samples).
+__device__ __forceinline__ int tile_samples(const Slab& s, int tile) { return min(s.samples, s.p.N - tile * s.samples); }
+
+// The values of this thread's channels out of one for each group, as pairs.
+template <int V>
+__device__ __forceinline__ void of_groups(const Pack& w, int D, const float* at, F2 (&out)[(V + 1) / 2]) {
+    if (w.rem + V <= D) { // one group
+        const float v = at[w.g];
+#pragma unroll
+        for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v, v);
+        return;
+    }
+    float v[(V + 1) / 2 * 2] = {};
+    int g = w.g, r = w.rem;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        v[i] = at[g];
+        if (++r == D) {
+            r = 0;
+            ++g;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v[2 * k], v[2 * k + 1]);
+}
+
+// weight and bias of this thread's channels
+template <int V>
+__device__ __forceinline__ void params_of(const Norm& p, const Pack& w, F2 (&weight)[(V + 1) / 2], F2 (&bias)[(V + 1) / 2]) {
+    float a[(V + 1) / 2 * 2] = {}, b[(V + 1) / 2 * 2] = {};
+    if (w.busy) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            a[i] = p.weight ? sa_param(p.weight, w.first + w.word * V + i, p.param_dtype) : 1.0f;
+            b[i] = p.bias ? sa_param(p.bias, w.first + w.word * V + i, p.param_dtype) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < (V + 1) / 2; ++k) {
+        weight[k] = f2(a[2 * k], a[2 * k + 1]);
+        bias[k] = f2(b[2 * k], b[2 * k + 1]);
+    }
+}
+
+// f(sample, group, first element or word, last + 1, whether there is such a group) for the groups of a tile, `lanes` threads each;
+// all threads of a warp call f together.
+template <class F>
+__device__ __forceinline__ void for_teams(const Slab& s, int samples, F&& f) {
+    const int teams = samples * s.groups, at_once = kThreads / s.lanes;
+    for (int t0 = 0; t0 < teams; t0 += at_once) {
+        const int t = min(t0 + (int)threadIdx.x / s.lanes, teams - 1);
+        const int sample = (int)s.by_groups.div((uint32_t)t);
+        f(sample, t - sample * s.groups, t, t0 + (int)threadIdx.x / s.lanes < teams);
+    }
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 4)
+sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    using Word = SaVec<T, V>;
+    extern __shared__ __align__(16) unsigned char memory[];
+    const size_t bytes = ((size_t)s.rows * s.pitch * sizeof(Word) + 15) / 16 * 16;
+    float* const centre = (float*)(memory + 2 * bytes); // [samples][groups] each: mean, rstd
+    float* const scale = centre + s.samples * s.groups;
+    const Pack w = pack_of<V>(s);
+    const Norm& p = s.p;
+    const int S = (int)p.S, D = p.D, width = s.pitch * V;
+    const long long step = (long long)s.row_lanes * p.C, base = (long long)w.row_lane * p.C + w.first + w.word * V;
+    const int own = w.row_lane * s.pitch + w.word, stride = s.row_lanes * s.pitch;
+    auto fetch = [&](int tile, int buffer) {
+        if (tile < s.tiles && w.busy) {
+            const T* from = x + (long long)tile * s.samples * S * p.C + base;
+            Word* to = (Word*)(memory + buffer * bytes) + own;
+            const int rows = tile_samples(s, tile) * S;
+#pragma unroll 4
+            for (int r = w.row_lane; r < rows; r += s.row_lanes, from += step, to += stride) fetch_row<T, V>(to, from);
+        }
+        end_of_stage();
+    };
+    fetch(w.first_tile, 0);
+    F2 weight[P], bias[P];
+    params_of<V>(p, w, weight, bias);
+    const float inv = 1.0f / ((float)S * (float)D);
+    int buffer = 0;
+    for (int tile = w.first_tile; tile < s.tiles; tile += s.blocks, buffer ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        fetch(tile + s.blocks, buffer ^ 1);
+        const Word* const data = (const Word*)(memory + buffer * bytes);
+        const int samples = tile_samples(s, tile);
+        for_teams(s, samples, [&](int sample, int g, int t, bool is) {
+            const T* const at = (const T*)data + sample * S * width + g * D;
+            const bool real = g < w.groups;
+            const int sub = threadIdx.x & (s.lanes - 1), count = real ? S * D : 0;
+            const float k0 = real ? sa_to_float(*at) : 0.0f;
+            float sum = 0.0f, m2 = 0.0f, m;
+            if (V > 1 && D % V == 0) {
+                const int words = D / V, n = count / V;
+                auto each = [&](float about, auto&& f) {
+                    const F2 c = f2(-about, -about);
+                    for (int e = sub; e < n; e += s.lanes) {
+                        const int row = (int)s.by_D.div((uint32_t)(e * V)); // place e lies in this row of the group
+                        const Word v = ((const Word*)at)[e + row * (s.pitch - words)];
+#pragma unroll
+                        for (int k = 0; k < P; ++k) f(pair_of(v, k) + c);
+                    }
+                };
+                F2 total = f2(0.0f, 0.0f), square = total;
+                each(k0, [&](F2 d) { total = total + d; });
+                float a, b;
+                split(total, a, b);
+                m = fmaf(lanes_sum(a + b, s.lanes), inv, k0);
+                each(m, [&](F2 d) { square = fma2(d, d, square); });
+                split(square, a, b);
+                m2 = lanes_sum(a + b, s.lanes);
+            } else {
+                auto each = [&](float about, auto&& f) {
+                    for (int e = sub; e < count; e += s.lanes) f(sa_to_float(at[e + (int)s.by_D.div((uint32_t)e) * (width - D)]) - about);
+                };
+                each(k0, [&](float d) { sum += d; });
+                m = fmaf(lanes_sum(sum, s.lanes), inv, k0);
+                each(m, [&](float d) { m2 = fmaf(d, d, m2); });
+                m2 = lanes_sum(m2, s.lanes);
+            }
+            if (is && real && sub == 0) {
+                const float rs = 1.0f / sqrtf(m2 * inv + p.eps);
+                centre[t] = m;
+                scale[t] = rs;
+                const long long to = ((long long)tile * s.samples + sample) * p.G + w.group0 + g;
+                mean[to] = m;
+                rstd[to] = rs;
+            }
+        });
+        __syncthreads();
+        if (!w.busy) continue;
+        T* to = out + (long long)tile * s.samples * S * p.C + base;
+        const Word* row = data + own;
+        const int rows = samples * S;
+        with_activation(p.silu, [&](auto silu) {
+#pragma unroll 2
+            for (int r = w.row_lane; r < rows; r += s.row_lanes, to += step, row += stride) {
+                Word v = *row;
+                const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
+                F2 m[P], rs[P];
+                of_groups<V>(w, D, centre + of, m);
+                of_groups<V>(w, D, scale + of, rs);
+#pragma unroll
+                for (int k = 0; k < P; ++k)
+                    set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + negative(m[k]), rs[k] * weight[k], bias[k])));
+                sa_store_stream<T, V>(to, v);
+            }
+        });
+    }
+}
+
+// `partial`: [blocks of a slab][C], each block's sums of (dz, dz u) over its samples; NULL: not wanted.  dz is kept in fp32 in
+// shared memory, so that the activation's derivative is worked out once.
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads, 3)
+sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
+                               float2* __restrict__ partial, const __grid_constant__ Slab s) {
+    constexpr int P = (V + 1) / 2;
+    using Word = SaVec<T, V>;
+    using Floats = SaVec<float, (V >= 4 ? 4 : V)>;
+    constexpr int kPer = V >= 4 ? 4 : V;
+    extern __shared__ __align__(16) unsigned char memory[];
+    const size_t bytes = ((size_t)s.rows * s.pitch * sizeof(Word) + 15) / 16 * 16;
+    const int teams = s.samples * s.groups, width = s.pitch * V;
+    float* const flow = (float*)(memory + 4 * bytes); // dz, as x lies; in the end the sums of the block
+    const size_t tile_floats = (size_t)s.rows * width, sum_floats = (size_t)(s.row_lanes + 1) / 2 * s.width * 2;
+    float* const weights = flow + ((tile_floats > sum_floats ? tile_floats : sum_floats) + 3) / 4 * 4; // [width]
+    float* const first = weights + (s.width + 3) / 4 * 4; // [teams] each: -rstd m1, -rstd^2 m2
+    float* const second = first + teams;
+    float* const stats = second + teams;                  // [2][teams] means, [2][teams] rstd
+    may_follow();
+    const Pack w = pack_of<V>(s);
+    const Norm& p = s.p;
+    const int S = (int)p.S, D = p.D;
+    const long long step = (long long)s.row_lanes * p.C, base = (long long)w.row_lane * p.C + w.first + w.word * V;
+    const int own = w.row_lane * s.pitch + w.word, stride = s.row_lanes * s.pitch;
+    auto fetch = [&](int tile, int buffer) {
+        if (tile < s.tiles) {
+            const int samples = tile_samples(s, tile), rows = samples * S;
+            if (w.busy) {
+                const long long at = (long long)tile * s.samples * S * p.C + base;
+                const T *from = x + at, *other = dout + at;
+                Word* to = (Word*)(memory + buffer * bytes) + own;
+                Word* beside = (Word*)(memory + (2 + buffer) * bytes) + own;
+#pragma unroll 2
+                for (int r = w.row_lane; r < rows; r += s.row_lanes, from += step, other += step, to += stride, beside += stride) {
+                    fetch_row<T, V>(to, from);
+                    fetch_row<T, V>(beside, other);
+                }
+            }
+            for (int t = threadIdx.x; t < samples * s.groups; t += kThreads) {
+                const int sample = (int)s.by_groups.div((uint32_t)t), g = t - sample * s.groups;
+                if (g >= w.groups) continue;
+                const long long at = ((long long)tile * s.samples + sample) * p.G + w.group0 + g;
+                fetch_row<float, 1>((SaVec<float, 1>*)(stats + buffer * teams + t), mean + at);
+                fetch_row<float, 1>((SaVec<float, 1>*)(stats + (2 + buffer) * teams + t), rstd + at);
+            }
+        }
+        end_of_stage();
+    };
+    fetch(w.first_tile, 0);
+    for (int j = threadIdx.x; j < w.channels; j += kThreads) weights[j] = p.weight ? sa_param(p.weight, w.first + j, p.param_dtype) : 1.0f;
+    F2 weight[P], bias[P], a0[P], a1[P];
+    params_of<V>(p, w, weight, bias);
+#pragma unroll
+    for (int k = 0; k < P; ++k) a0[k] = a1[k] = f2(0.0f, 0.0f);
+    const float inv = 1.0f / ((float)S * (float)D);
+    int buffer = 0;
+    for (int tile = w.first_tile; tile < s.tiles; tile += s.blocks, buffer ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        fetch(tile + s.blocks, buffer ^ 1);
+        const Word* const data = (const Word*)(memory + buffer * bytes);
+        const Word* const grad = (const Word*)(memory + (2 + buffer) * bytes);
+        const float *const centre = stats + buffer * teams, *const scale = stats + (2 + buffer) * teams;
+        const int samples = tile_samples(s, tile), rows = samples * S;
+        if (w.busy) {
+            with_activation(p.silu, [&](auto silu) {
+                int at = own;
+                for (int r = w.row_lane; r < rows; r += s.row_lanes, at += stride) {
+                    const Word v = data[at], d = grad[at];
+                    const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
+                    F2 m[P], rs[P];
+                    of_groups<V>(w, D, centre + of, m);
+                    of_groups<V>(w, D, scale + of, rs);
+                    float dzs[2 * P];
+#pragma unroll
+                    for (int k = 0; k < P; ++k) {
+                        const F2 u = (pair_of(v, k) + negative(m[k])) * rs[k];
+                        const F2 dz = through_activation2<T, silu.value>(pair_of(d, k), fma2(u, weight[k], bias[k]));
+                        a0[k] = a0[k] + dz;
+                        a1[k] = fma2(dz, u, a1[k]);
+                        split(dz, dzs[2 * k], dzs[2 * k + 1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < V / kPer; ++k) {
+                        Floats f;
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) f.e[i] = dzs[k * kPer + i];
+                        *(Floats*)(flow + (size_t)at * V + k * kPer) = f;
+                    }
+                }
+            });
+        }
+        __syncthreads();
+        for_teams(s, samples, [&](int sample, int g, int t, bool is) {
+            const bool real = g < w.groups;
+            const int sub = threadIdx.x & (s.lanes - 1), count = real ? S * D : 0, from = sample * S * width + g * D;
+            const T* const at = (const T*)data + from;
+            const float *const dz = flow + from, *const wg = weights + g * D;
+            const float m = real ? centre[t] : 0.0f, rs = real ? scale[t] : 0.0f;
+            float t1 = 0.0f, t2 = 0.0f;
+            if (V > 1 && D % V == 0) {
+                const int words = D / V, n = count / V;
+                F2 s1 = f2(0.0f, 0.0f), s2 = s1;
+                for (int e = sub; e < n; e += s.lanes) {
+                    const int row = (int)s.by_D.div((uint32_t)(e * V)), place = e + row * (s.pitch - words);
+                    const Word v = ((const Word*)at)[place];
+                    const float *const z = dz + place * V, *const we = wg + (e - row * words) * V;
+#pragma unroll
+                    for (int k = 0; k < V / kPer; ++k) {
+                        const Floats f = *(const Floats*)(z + k * kPer), fw = *(const Floats*)(we + k * kPer);
+#pragma unroll
+                        for (int i = 0; i < kPer / 2; ++i) {
+                            const F2 q = f2(f.e[2 * i], f.e[2 * i + 1]) * f2(fw.e[2 * i], fw.e[2 * i + 1]);
+                            s1 = s1 + q;
+                            s2 = fma2(q, pair_of(v, k * (kPer / 2) + i) + f2(-m, -m), s2);
+                        }
+                    }
+                }
+                float a, b;
+                split(s1, a, b);
+                t1 = a + b;
+                split(s2, a, b);
+                t2 = a + b;
+            } else {
+                for (int e = sub; e < count; e += s.lanes) {
+                    const int row = (int)s.by_D.div((uint32_t)e), place = e + row * (width - D);
+                    const float q = dz[place] * wg[e - row * D];
+                    t1 += q;
+                    t2 = fmaf(q, sa_to_float(at[place]) - m, t2);
+                }
+            }
+            t1 = lanes_sum(t1, s.lanes) * inv;
+            t2 = lanes_sum(t2, s.lanes) * inv;
+            if (is && real && sub == 0) { // dx = (w rstd) dz - rstd m1 - (x - mean) rstd^2 m2, m2 = rstd t2
+                first[t] = -rs * t1;
+                second[t] = -rs * (rs * (rs * t2));
+            }
+        });
+        __syncthreads();
+        if (!w.busy) continue;
+        T* to = dx + (long long)tile * s.samples * S * p.C + base;
+        int at = own;
+        for (int r = w.row_lane; r < rows; r += s.row_lanes, at += stride, to += step) {
+            Word v = data[at];
+            const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
+            F2 m[P], rs[P], m1[P], m2[P];
+            of_groups<V>(w, D, centre + of, m);
+            of_groups<V>(w, D, scale + of, rs);
+            of_groups<V>(w, D, first + of, m1);
+            of_groups<V>(w, D, second + of, m2);
+            F2 dz[P];
+            shared_pairs<V>(dz, flow + (size_t)at * V);
+#pragma unroll
+            for (int k = 0; k < P; ++k)
+                set_pair(v, k, fma2(pair_of(v, k) + negative(m[k]), m2[k], fma2(rs[k] * weight[k], dz[k], m1[k])));
+            sa_store_stream<T, V>(to, v);
+        }
+    }
+    if (!partial) return;
+    __syncthreads(); // dz becomes the sums
+    Place place{};
+    place.word = w.word;
+    place.row_lane = w.row_lane;
+    block_sums<V>(s, place, (float2*)flow, a0, a1);
+    for (int j = threadIdx.x; j < w.channels; j += kThreads)
+        partial[(long long)w.first_tile * p.C + w.first + j] = channel_sum<V>(s, (const float2*)flow, j);
+}
+
+// ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
 // Threads that share a channel's column of `lanes` values: the column is added up in lanes / shares steps, the shares in
@@ -1222,10 +1582,53 @@ double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors
     return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 6.0;
 }
 
+// The same for tiles of short samples.
+double packed_time(const Norm& p, const Slab& s, int V, int esize, int tensors) {
+    const double mb = (double)p.N * (double)p.S * (double)p.C * esize * (tensors + 1) * 1e-6;
+    return 4.0 + mb / 3.0;
+}
+
 // The same for the way of long samples: three or four launches (fitted to 0.2-134 MB of x; within 20 %).
 double streamed_time(const Norm& p, int V, int esize, int tensors) {
     const double mb = (double)p.N * (double)p.S * (double)p.C * esize * 1e-6 * (V * esize == 16 ? 1.0 : V * esize == 4 ? 4.0 : 8.0);
     return tensors == 1 ? 17.0 + 0.45 * mb : 31.0 + 0.75 * mb;
+}
+
+// Short samples: tiles of whole samples, 16 KiB of x (half of that backward), fewer where that leaves SMs without any.
+bool pack(const Norm& p, int V, int esize, int tensors, int unit, Slab* best) {
+    const long long cap = 16 * 1024 / tensors, column = p.S * p.D * esize; // bytes of a tile, of a group of a sample
+    long long groups = std::min(std::min(cap / column, 256ll * V / p.D) / unit * unit, (long long)p.G);
+    if (groups < 1) return false;
+    Slab s{};
+    s.p = p;
+    s.slabs = (int)((p.G + groups - 1) / groups);
+    groups = ((p.G + s.slabs - 1) / s.slabs + unit - 1) / unit * unit;
+    s.slabs = (int)((p.G + groups - 1) / groups);
+    s.groups = (int)groups;
+    s.width = s.groups * p.D;
+    s.words = s.width / V;
+    s.pitch = s.words | 1;
+    s.threads = kThreads;
+    s.row_lanes = kThreads / s.words;
+    s.samples = (int)std::max(1ll, std::min({cap / (column * groups), (long long)p.N, (long long)p.N * s.slabs / (148 * 4)}));
+    s.rows = s.samples * (int)p.S;
+    s.tiles = (p.N + s.samples - 1) / s.samples;
+    const int at_once = std::min(s.tiles, std::max(1, 148 * (tensors == 1 ? 4 : 3) / s.slabs)), each = (s.tiles + at_once - 1) / at_once;
+    s.blocks = (s.tiles + each - 1) / each;
+    const int teams = s.samples * s.groups, items = (int)p.S * p.D / (p.D % V ? 1 : V), half = (s.row_lanes + 1) / 2;
+    for (s.lanes = 1; s.lanes < 32 && s.lanes * 2 <= items && s.lanes * teams < kThreads;) s.lanes *= 2;
+    s.parts = shares(half, kThreads / s.width);
+    s.by_words = divisor((uint32_t)s.words);
+    s.by_width = divisor((uint32_t)s.width);
+    s.by_D = divisor((uint32_t)p.D);
+    s.by_S = divisor((uint32_t)p.S);
+    s.by_groups = divisor((uint32_t)s.groups);
+    const size_t words = (size_t)s.rows * s.pitch, bytes = (words * V * esize + 15) / 16 * 16;
+    if (tensors == 1) s.shared = 2 * bytes + sizeof(float) * 2 * teams;
+    else s.shared = 4 * bytes + sizeof(float) * ((std::max(words * V, (size_t)half * s.width * 2) + 3) / 4 * 4 + (s.width + 3) / 4 * 4 + 6 * (size_t)teams);
+    if (s.shared > kMostShared || (long long)s.slabs * s.blocks > 0x7fffffffll) return false;
+    *best = s;
+    return true;
 }
 
 // Whether the groups of a sample are to be resident, and how: every slab width (multiples of the narrowest one that is whole
@@ -1237,6 +1640,14 @@ bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     while ((unit * (long long)p.D) % V) ++unit;
     double least = streamed_time(p, V, esize, tensors);
     bool found = false;
+    Slab packed{};
+    if (pack(p, V, esize, tensors, unit, &packed)) {
+        if (const double time = packed_time(p, packed, V, esize, tensors); time < least) {
+            least = time;
+            *best = packed;
+            found = true;
+        }
+    }
     for (int m = 1; m == 1 || unit * (m - 1) < p.G; ++m) {
         const int groups = unit * m < p.G ? unit * m : p.G;
         const long long width = (long long)groups * p.D;
@@ -1389,7 +1800,11 @@ size_t ring_bytes(size_t tile) {
 template <class T, int V>
 cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream, int& launched) {
     Slab s;
-    if (p.fold == 1 && plan_resident(p, V, sizeof(T), 1, &s))
+    const bool planned = p.fold == 1 && plan_resident(p, V, sizeof(T), 1, &s);
+    if (planned && s.samples)
+        return launch(sa_norm_packed_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream, launched, (T*)out,
+                      (const T*)x, mean, rstd, s);
+    if (planned)
         return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, launched, (T*)out, (const T*)x, mean, rstd, s);
     s = cut(p, V);
     const size_t params = sizeof(float) * 3 * (size_t)s.width;
@@ -1410,7 +1825,14 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     auto join_params = [&](const float2* sums, int count, int C) {
         return launch(sa_norm_backward_params_kernel, (C + 31) / 32, 1024, 0, true, stream, launched, sums, dweight, dbias, count, C, p.param_dtype);
     };
-    if (p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s)) {
+    const bool planned = p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s);
+    if (planned && s.samples) {
+        float2* const sums = dweight || dbias ? (float2*)workspace : nullptr; // [blocks of a slab][C]
+        const cudaError_t e = launch(sa_norm_packed_backward_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream,
+                                     launched, (T*)dx, (const T*)dout, (const T*)x, mean, rstd, sums, s);
+        return e != cudaSuccess || !sums ? e : join_params(sums, s.blocks, (int)p.C);
+    }
+    if (planned) {
         float2* const sums = p.N > 1 && (dweight || dbias) ? (float2*)workspace : nullptr;
         const cudaError_t e = launch_clusters(sa_norm_resident_backward_kernel<T, V>, s, stream, launched, (T*)dx, (const T*)dout, (const T*)x,
                                               mean, rstd, sums, p.N > 1 ? nullptr : dweight, p.N > 1 ? nullptr : dbias, s);
@@ -1466,7 +1888,10 @@ size_t sa_group_norm_workspace(const sideaware_group_norm_t& sh, bool backward) 
         if (sh.C % V) continue;
         const Norm p = describe(sh, nullptr, nullptr);
         Slab s;
-        const long long entries = plan_resident(p, V, e, backward ? 2 : 1, &s) ? (backward && sh.N > 1 ? (long long)sh.N * sh.C : 0) : streamed(p, V);
+        long long entries;
+        if (!plan_resident(p, V, e, backward ? 2 : 1, &s)) entries = streamed(p, V);
+        else if (!backward) entries = 0;
+        else entries = s.samples ? (long long)s.blocks * sh.C : sh.N > 1 ? (long long)sh.N * sh.C : 0;
         if (entries > most) most = entries;
     }
     Norm p = describe(sh, nullptr, nullptr);

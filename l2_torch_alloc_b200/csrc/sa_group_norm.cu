@@ -10,12 +10,14 @@
 // Golub and LeVeque (1983), all in fp32: no cancellation however far the mean is from zero.  All sums go through fixed trees
 // (no atomics): the same inputs give the same bits.
 //
-// Two ways, chosen by search_resident below:
+// Three ways, chosen by estimated times in search_plan below:
 //  * resident: a thread-block cluster owns some neighbouring groups of one sample, all rows of them lie in the shared
 //    memory of its blocks, which exchange their statistics through distributed shared memory.  One launch, each element
 //    is read once and written once.
 //  * streamed, for samples too long for that: partial statistics of runs of rows, joining them, applying them; three
 //    launches that overlap, x is read twice (a part of it from L2).
+//  * packed, for many short samples (a token's channels, a small image) and for little work: a block has several whole samples
+//    in its shared memory at a time and goes on to the next ones, which are already on their way.
 //
 // Bound and measured on a B200 (device time of a call, three sets of inputs in turn):
 //  * resident: the phases of a block follow one another, and each moves about 4 TB/s alone.  8 x 4096 x 320 bf16: 16.7 us (6.4
@@ -24,7 +26,8 @@
 //    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.2 us.
 //  * streamed: HBM.  2 x 262144 x 128 bf16: 74.5 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
 //    us for the copy-like second pass.
-//  * small: latency.  1 x 64 x 1280 bf16: 5 us, of which 0.9 is the HBM's latency and 1.5 the joining of statistics.
+//  * packed: instructions, about 280 of a warp for a word of each lane forward and 600 backward.  16384 x 1 x 2048 bf16: 48 us
+//    and 137 us (resident or streamed: 580 and 1080); 1 x 64 x 1280 bf16: 4.0 us, which is latency (resident 5.1).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1153,6 +1156,7 @@ struct Pack {
     long long first;      // first channel of the slab
     int group0;           // first group of the slab
     int g, rem;           // group of the thread's first channel in the slab, place in that group
+    int next, edge;       // the group after it, if the word reaches that far; first channel of the word that belongs to it
     bool busy;            // has a word
 };
 
@@ -1169,33 +1173,53 @@ __device__ __forceinline__ Pack pack_of(const Slab& s) {
     w.channels = (int)min((long long)s.width, s.p.C - w.first);
     w.g = (int)s.by_D.div((uint32_t)(w.word * V));
     w.rem = w.word * V - w.g * s.p.D;
+    w.edge = s.p.D - w.rem;
+    w.next = w.g + (w.edge < V ? 1 : 0);
     w.busy = w.row_lane < s.row_lanes && w.word * V < w.channels;
     return w;
 }
 // Rows of a tile (they follow one another in memory, whole samples).
 __device__ __forceinline__ int tile_samples(const Slab& s, int tile) { return min(s.samples, s.p.N - tile * s.samples); }
 
-// The values of this thread's channels out of one for each group, as pairs.
+// The values of this thread's channels out of one for each group, as pairs.  Which way is the same for all threads: words inside
+// groups, words with at most one border between pairs, or any.
 template <int V>
 __device__ __forceinline__ void of_groups(const Pack& w, int D, const float* at, F2 (&out)[(V + 1) / 2]) {
-    if (w.rem + V <= D) { // one group
+    if (D % V == 0) {
         const float v = at[w.g];
 #pragma unroll
         for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v, v);
-        return;
-    }
-    float v[(V + 1) / 2 * 2] = {};
-    int g = w.g, r = w.rem;
+    } else if (D >= V && D % 2 == 0) {
+        const float v0 = at[w.g], v1 = at[w.next];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        v[i] = at[g];
-        if (++r == D) {
-            r = 0;
-            ++g;
+        for (int k = 0; k < (V + 1) / 2; ++k) {
+            const float v = 2 * k < w.edge ? v0 : v1;
+            out[k] = f2(v, v);
         }
-    }
+    } else {
+        float v[(V + 1) / 2 * 2] = {};
+        int g = w.g, r = w.rem;
 #pragma unroll
-    for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v[2 * k], v[2 * k + 1]);
+        for (int i = 0; i < V; ++i) {
+            v[i] = at[g];
+            if (++r == D) {
+                r = 0;
+                ++g;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v[2 * k], v[2 * k + 1]);
+    }
+}
+
+// Elements of an item, what a thread takes of a group at a time: as many as divide the group, up to a word.
+// f(std::integral_constant) for that number, the same for all threads.
+template <int V, class F>
+__device__ __forceinline__ void with_items(int D, F&& f) {
+    if (D % V == 0) f(std::integral_constant<int, V>());
+    else if (V > 4 && D % 4 == 0) f(std::integral_constant<int, (V > 4 ? 4 : V)>());
+    else if (V > 2 && D % 2 == 0) f(std::integral_constant<int, (V > 2 ? 2 : V)>());
+    else f(std::integral_constant<int, 1>());
 }
 
 // weight and bias of this thread's channels
@@ -1229,7 +1253,7 @@ __device__ __forceinline__ void for_teams(const Slab& s, int samples, F&& f) {
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, 3)
 sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     using Word = SaVec<T, V>;
@@ -1268,35 +1292,43 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
             const bool real = g < w.groups;
             const int sub = threadIdx.x & (s.lanes - 1), count = real ? S * D : 0;
             const float k0 = real ? sa_to_float(*at) : 0.0f;
-            float sum = 0.0f, m2 = 0.0f, m;
-            if (V > 1 && D % V == 0) {
-                const int words = D / V, n = count / V;
+            float m = 0.0f, m2 = 0.0f;
+            with_items<V>(D, [&](auto size) {
+                constexpr int W = size.value;
                 auto each = [&](float about, auto&& f) {
                     const F2 c = f2(-about, -about);
-                    for (int e = sub; e < n; e += s.lanes) {
-                        const int row = (int)s.by_D.div((uint32_t)(e * V)); // place e lies in this row of the group
-                        const Word v = ((const Word*)at)[e + row * (s.pitch - words)];
+#pragma unroll 2
+                    for (int e = sub * W; e < count; e += s.lanes * W) {
+                        const SaVec<T, W> v = sa_load<T, W>(at + e + (int)s.by_D.div((uint32_t)e) * (width - D));
+                        if constexpr (W == 1) f(f2(sa_to_float(v.e[0]) - about, 0.0f));
+                        else {
 #pragma unroll
-                        for (int k = 0; k < P; ++k) f(pair_of(v, k) + c);
+                            for (int k = 0; k < W / 2; ++k) f(pair_of(v, k) + c);
+                        }
                     }
                 };
-                F2 total = f2(0.0f, 0.0f), square = total;
-                each(k0, [&](F2 d) { total = total + d; });
-                float a, b;
-                split(total, a, b);
-                m = fmaf(lanes_sum(a + b, s.lanes), inv, k0);
-                each(m, [&](F2 d) { square = fma2(d, d, square); });
-                split(square, a, b);
-                m2 = lanes_sum(a + b, s.lanes);
-            } else {
-                auto each = [&](float about, auto&& f) {
-                    for (int e = sub; e < count; e += s.lanes) f(sa_to_float(at[e + (int)s.by_D.div((uint32_t)e) * (width - D)]) - about);
+                auto all = [&](F2 v) {
+                    float a, b;
+                    split(v, a, b);
+                    return lanes_sum(a + b, s.lanes);
                 };
-                each(k0, [&](float d) { sum += d; });
-                m = fmaf(lanes_sum(sum, s.lanes), inv, k0);
-                each(m, [&](float d) { m2 = fmaf(d, d, m2); });
-                m2 = lanes_sum(m2, s.lanes);
-            }
+                F2 total = f2(0.0f, 0.0f), square = total;
+                each(k0, [&](F2 d) {
+                    total = total + d;
+                    square = fma2(d, d, square);
+                });
+                const float sum = all(total), squares = all(square), off = sum * inv;
+                m = k0 + off;
+                m2 = fmaf(-sum, off, squares);
+                // the first element is far out: what cancels would be 16 times what is left, so once more about the mean
+                const bool again = !(squares <= 16.0f * m2);
+                if (__any_sync(0xffffffffu, again)) {
+                    square = f2(0.0f, 0.0f);
+                    each(m, [&](F2 d) { square = fma2(d, d, square); });
+                    const float exact = all(square);
+                    if (again) m2 = exact;
+                }
+            });
             if (is && real && sub == 0) {
                 const float rs = 1.0f / sqrtf(m2 * inv + p.eps);
                 centre[t] = m;
@@ -1311,29 +1343,37 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
         T* to = out + (long long)tile * s.samples * S * p.C + base;
         const Word* row = data + own;
         const int rows = samples * S;
+        F2 m[P], a[P];
+        int have = -1;
         with_activation(p.silu, [&](auto silu) {
-#pragma unroll 2
             for (int r = w.row_lane; r < rows; r += s.row_lanes, to += step, row += stride) {
                 Word v = *row;
-                const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
-                F2 m[P], rs[P];
-                of_groups<V>(w, D, centre + of, m);
-                of_groups<V>(w, D, scale + of, rs);
+                if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) { // the next sample
+                    have = of;
+                    of_groups<V>(w, D, centre + of, m);
+                    of_groups<V>(w, D, scale + of, a);
 #pragma unroll
-                for (int k = 0; k < P; ++k)
-                    set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + negative(m[k]), rs[k] * weight[k], bias[k])));
+                    for (int k = 0; k < P; ++k) {
+                        m[k] = negative(m[k]);
+                        a[k] = a[k] * weight[k];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], bias[k])));
                 sa_store_stream<T, V>(to, v);
             }
         });
     }
 }
 
-// `partial`: [blocks of a slab][C], each block's sums of (dz, dz u) over its samples; NULL: not wanted.  dz is kept in fp32 in
+// `partial`: [blocks of a slab][C], each block's sums of (dz, dz u) over its samples; NULL: there is one block, dweight and
+// dbias are written here.  dz is kept in fp32 in
 // shared memory, so that the activation's derivative is worked out once.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 2)
 sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
-                               float2* __restrict__ partial, const __grid_constant__ Slab s) {
+                               float2* __restrict__ partial, void* __restrict__ dweight, void* __restrict__ dbias,
+                               const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     using Word = SaVec<T, V>;
     using Floats = SaVec<float, (V >= 4 ? 4 : V)>;
@@ -1344,7 +1384,8 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
     float* const flow = (float*)(memory + 4 * bytes); // dz, as x lies; in the end the sums of the block
     const size_t tile_floats = (size_t)s.rows * width, sum_floats = (size_t)(s.row_lanes + 1) / 2 * s.width * 2;
     float* const weights = flow + ((tile_floats > sum_floats ? tile_floats : sum_floats) + 3) / 4 * 4; // [width]
-    float* const first = weights + (s.width + 3) / 4 * 4; // [teams] each: -rstd m1, -rstd^2 m2
+    float* const biases = weights + (s.width + 3) / 4 * 4;
+    float* const first = biases + (s.width + 3) / 4 * 4;  // [teams] each: -rstd m1, -rstd^2 m2
     float* const second = first + teams;
     float* const stats = second + teams;                  // [2][teams] means, [2][teams] rstd
     may_follow();
@@ -1378,9 +1419,11 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
         end_of_stage();
     };
     fetch(w.first_tile, 0);
-    for (int j = threadIdx.x; j < w.channels; j += kThreads) weights[j] = p.weight ? sa_param(p.weight, w.first + j, p.param_dtype) : 1.0f;
-    F2 weight[P], bias[P], a0[P], a1[P];
-    params_of<V>(p, w, weight, bias);
+    for (int j = threadIdx.x; j < s.width; j += kThreads) {
+        weights[j] = p.weight && j < w.channels ? sa_param(p.weight, w.first + j, p.param_dtype) : 1.0f;
+        biases[j] = p.bias && j < w.channels ? sa_param(p.bias, w.first + j, p.param_dtype) : 0.0f;
+    }
+    F2 a0[P], a1[P];
 #pragma unroll
     for (int k = 0; k < P; ++k) a0[k] = a1[k] = f2(0.0f, 0.0f);
     const float inv = 1.0f / ((float)S * (float)D);
@@ -1395,13 +1438,18 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
         const int samples = tile_samples(s, tile), rows = samples * S;
         if (w.busy) {
             with_activation(p.silu, [&](auto silu) {
-                int at = own;
+                int at = own, have = -1;
+                F2 m[P], rs[P];
                 for (int r = w.row_lane; r < rows; r += s.row_lanes, at += stride) {
                     const Word v = data[at], d = grad[at];
-                    const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
-                    F2 m[P], rs[P];
-                    of_groups<V>(w, D, centre + of, m);
-                    of_groups<V>(w, D, scale + of, rs);
+                    if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) { // the next sample
+                        have = of;
+                        of_groups<V>(w, D, centre + of, m);
+                        of_groups<V>(w, D, scale + of, rs);
+                    }
+                    F2 weight[P], bias[P];
+                    shared_pairs<V>(weight, weights + w.word * V);
+                    shared_pairs<V>(bias, biases + w.word * V);
                     float dzs[2 * P];
 #pragma unroll
                     for (int k = 0; k < P; ++k) {
@@ -1429,21 +1477,28 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
             const float *const dz = flow + from, *const wg = weights + g * D;
             const float m = real ? centre[t] : 0.0f, rs = real ? scale[t] : 0.0f;
             float t1 = 0.0f, t2 = 0.0f;
-            if (V > 1 && D % V == 0) {
-                const int words = D / V, n = count / V;
+            with_items<V>(D, [&](auto size) {
+                constexpr int W = size.value;
+                constexpr int kPiece = W >= 4 ? 4 : W;
                 F2 s1 = f2(0.0f, 0.0f), s2 = s1;
-                for (int e = sub; e < n; e += s.lanes) {
-                    const int row = (int)s.by_D.div((uint32_t)(e * V)), place = e + row * (s.pitch - words);
-                    const Word v = ((const Word*)at)[place];
-                    const float *const z = dz + place * V, *const we = wg + (e - row * words) * V;
+#pragma unroll 2
+                for (int e = sub * W; e < count; e += s.lanes * W) {
+                    const int row = (int)s.by_D.div((uint32_t)e), place = e + row * (width - D);
+                    const SaVec<T, W> v = sa_load<T, W>(at + place);
 #pragma unroll
-                    for (int k = 0; k < V / kPer; ++k) {
-                        const Floats f = *(const Floats*)(z + k * kPer), fw = *(const Floats*)(we + k * kPer);
+                    for (int k = 0; k < W; k += kPiece) {
+                        const auto z = sa_load<float, kPiece>(dz + place + k), we = sa_load<float, kPiece>(wg + e - row * D + k);
+                        if constexpr (W == 1) {
+                            const float q = z.e[0] * we.e[0];
+                            s1 = s1 + f2(q, 0.0f);
+                            s2 = s2 + f2(q * (sa_to_float(v.e[0]) - m), 0.0f);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < kPer / 2; ++i) {
-                            const F2 q = f2(f.e[2 * i], f.e[2 * i + 1]) * f2(fw.e[2 * i], fw.e[2 * i + 1]);
-                            s1 = s1 + q;
-                            s2 = fma2(q, pair_of(v, k * (kPer / 2) + i) + f2(-m, -m), s2);
+                            for (int i = 0; i < kPiece / 2; ++i) {
+                                const F2 q = f2(z.e[2 * i], z.e[2 * i + 1]) * f2(we.e[2 * i], we.e[2 * i + 1]);
+                                s1 = s1 + q;
+                                s2 = fma2(q, pair_of(v, k / 2 + i) + f2(-m, -m), s2);
+                            }
                         }
                     }
                 }
@@ -1452,14 +1507,7 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
                 t1 = a + b;
                 split(s2, a, b);
                 t2 = a + b;
-            } else {
-                for (int e = sub; e < count; e += s.lanes) {
-                    const int row = (int)s.by_D.div((uint32_t)e), place = e + row * (width - D);
-                    const float q = dz[place] * wg[e - row * D];
-                    t1 += q;
-                    t2 = fmaf(q, sa_to_float(at[place]) - m, t2);
-                }
-            }
+            });
             t1 = lanes_sum(t1, s.lanes) * inv;
             t2 = lanes_sum(t2, s.lanes) * inv;
             if (is && real && sub == 0) { // dx = (w rstd) dz - rstd m1 - (x - mean) rstd^2 m2, m2 = rstd t2
@@ -1470,31 +1518,42 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
         __syncthreads();
         if (!w.busy) continue;
         T* to = dx + (long long)tile * s.samples * S * p.C + base;
-        int at = own;
+        int at = own, have = -1;
+        F2 m[P], a[P], m1[P], m2[P];
         for (int r = w.row_lane; r < rows; r += s.row_lanes, at += stride, to += step) {
             Word v = data[at];
-            const int of = (int)s.by_S.div((uint32_t)r) * s.groups;
-            F2 m[P], rs[P], m1[P], m2[P];
-            of_groups<V>(w, D, centre + of, m);
-            of_groups<V>(w, D, scale + of, rs);
-            of_groups<V>(w, D, first + of, m1);
-            of_groups<V>(w, D, second + of, m2);
+            if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) {
+                have = of;
+                F2 weight[P];
+                shared_pairs<V>(weight, weights + w.word * V);
+                of_groups<V>(w, D, centre + of, m);
+                of_groups<V>(w, D, scale + of, a);
+                of_groups<V>(w, D, first + of, m1);
+                of_groups<V>(w, D, second + of, m2);
+#pragma unroll
+                for (int k = 0; k < P; ++k) a[k] = a[k] * weight[k];
+            }
             F2 dz[P];
             shared_pairs<V>(dz, flow + (size_t)at * V);
 #pragma unroll
-            for (int k = 0; k < P; ++k)
-                set_pair(v, k, fma2(pair_of(v, k) + negative(m[k]), m2[k], fma2(rs[k] * weight[k], dz[k], m1[k])));
+            for (int k = 0; k < P; ++k) set_pair(v, k, fma2(pair_of(v, k) + negative(m[k]), m2[k], fma2(a[k], dz[k], m1[k])));
             sa_store_stream<T, V>(to, v);
         }
     }
-    if (!partial) return;
+    if (!partial && !dweight && !dbias) return;
     __syncthreads(); // dz becomes the sums
     Place place{};
     place.word = w.word;
     place.row_lane = w.row_lane;
     block_sums<V>(s, place, (float2*)flow, a0, a1);
-    for (int j = threadIdx.x; j < w.channels; j += kThreads)
-        partial[(long long)w.first_tile * p.C + w.first + j] = channel_sum<V>(s, (const float2*)flow, j);
+    for (int j = threadIdx.x; j < w.channels; j += kThreads) {
+        const float2 t = channel_sum<V>(s, (const float2*)flow, j);
+        if (partial) partial[(long long)w.first_tile * p.C + w.first + j] = t;
+        else {
+            if (dbias) sa_set_param(dbias, w.first + j, p.param_dtype, t.x);
+            if (dweight) sa_set_param(dweight, w.first + j, p.param_dtype, t.y);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1582,21 +1641,31 @@ double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors
     return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 6.0;
 }
 
-// The same for tiles of short samples.
-double packed_time(const Norm& p, const Slab& s, int V, int esize, int tensors) {
-    const double mb = (double)p.N * (double)p.S * (double)p.C * esize * (tensors + 1) * 1e-6;
-    return 4.0 + mb / 3.0;
+// Blocks of the packed kernels that their registers let an SM have.
+int packed_on_sm(int tensors) { return tensors == 1 ? 3 : 2; }
+
+// The same for tiles of short samples: instructions, of the SM with the most tiles or of a block alone (fitted to 20 shapes, with
+// 1,000 to 134 million elements; the choice took at most 5 % longer than the better way).
+double packed_time(const Norm& p, const Slab& s, int V, int tensors) {
+    const double each = std::ceil((double)s.tiles / s.blocks), on_sm = std::ceil((double)s.slabs * s.blocks / 148);
+    const double thousands = s.rows * s.width * 1e-3 * (V == 8 ? 1.0 : V == 4 ? 1.7 : 2.4) * (p.D % V ? 1.3 : 1.0);
+    const double most = std::min(on_sm, (double)packed_on_sm(tensors)), rounds = std::ceil(on_sm / most);
+    if (tensors == 1) return 3.0 + rounds * each * (0.4 + thousands * std::max(0.3, 0.18 * most));
+    return 5.6 + rounds * each * (0.7 + thousands * std::max(0.5, 0.38 * most));
 }
 
 // The same for the way of long samples: three or four launches (fitted to 0.2-134 MB of x; within 20 %).
 double streamed_time(const Norm& p, int V, int esize, int tensors) {
     const double mb = (double)p.N * (double)p.S * (double)p.C * esize * 1e-6 * (V * esize == 16 ? 1.0 : V * esize == 4 ? 4.0 : 8.0);
-    return tensors == 1 ? 17.0 + 0.45 * mb : 31.0 + 0.75 * mb;
+    // many samples are many blocks, of the kernel that joins as well
+    const double blocks = (double)p.N * std::ceil((double)p.C / V / kThreads);
+    const double joins = (double)p.N * (tensors == 1 ? p.G / 8.0 : std::ceil((double)p.C / 32) / 2);
+    return (tensors == 1 ? 17.0 + 0.45 * mb : 31.0 + 0.75 * mb) + blocks / (148 * 3) * 8.0 + joins / 148 * 3.0;
 }
 
-// Short samples: tiles of whole samples, 16 KiB of x (half of that backward), fewer where that leaves SMs without any.
-bool pack(const Norm& p, int V, int esize, int tensors, int unit, Slab* best) {
-    const long long cap = 16 * 1024 / tensors, column = p.S * p.D * esize; // bytes of a tile, of a group of a sample
+// Short samples: tiles of whole samples with up to `cap` bytes of x, fewer where that leaves SMs without any.
+bool pack(const Norm& p, int V, int esize, int tensors, int unit, int cap, Slab* best) {
+    const long long column = p.S * p.D * esize; // bytes of a group of a sample
     long long groups = std::min(std::min(cap / column, 256ll * V / p.D) / unit * unit, (long long)p.G);
     if (groups < 1) return false;
     Slab s{};
@@ -1610,39 +1679,47 @@ bool pack(const Norm& p, int V, int esize, int tensors, int unit, Slab* best) {
     s.pitch = s.words | 1;
     s.threads = kThreads;
     s.row_lanes = kThreads / s.words;
-    s.samples = (int)std::max(1ll, std::min({cap / (column * groups), (long long)p.N, (long long)p.N * s.slabs / (148 * 4)}));
+    s.parts = shares((s.row_lanes + 1) / 2, kThreads / s.width);
+    const int on_sm = packed_on_sm(tensors);
+    const size_t most = tensors == 1 ? 75 * 1024 : 113 * 1024; // for three and two blocks
+    s.samples = (int)std::max(1ll, std::min({cap / (column * groups), (long long)p.N, (long long)p.N * s.slabs / (148 * on_sm)}));
+    for (;; --s.samples) {
+        const size_t words = (size_t)s.samples * p.S * s.pitch, bytes = (words * V * esize + 15) / 16 * 16, teams = (size_t)s.samples * s.groups;
+        if (tensors == 1) s.shared = 2 * bytes + sizeof(float) * 2 * teams;
+        else
+            s.shared = 4 * bytes + sizeof(float) * ((std::max(words * V, (size_t)(s.row_lanes + 1) / 2 * s.width * 2) + 3) / 4 * 4 +
+                                                    (s.width + 3) / 4 * 4 * 2 + 6 * teams);
+        if (s.shared <= most || s.samples == 1) break;
+    }
+    if (s.shared > kMostShared) return false;
     s.rows = s.samples * (int)p.S;
     s.tiles = (p.N + s.samples - 1) / s.samples;
-    const int at_once = std::min(s.tiles, std::max(1, 148 * (tensors == 1 ? 4 : 3) / s.slabs)), each = (s.tiles + at_once - 1) / at_once;
+    const int at_once = std::min(s.tiles, std::max(1, 148 * on_sm / s.slabs)), each = (s.tiles + at_once - 1) / at_once;
     s.blocks = (s.tiles + each - 1) / each;
-    const int teams = s.samples * s.groups, items = (int)p.S * p.D / (p.D % V ? 1 : V), half = (s.row_lanes + 1) / 2;
-    for (s.lanes = 1; s.lanes < 32 && s.lanes * 2 <= items && s.lanes * teams < kThreads;) s.lanes *= 2;
-    s.parts = shares(half, kThreads / s.width);
+    const int items = (int)p.S * p.D / (p.D % V == 0 ? V : p.D % 4 == 0 && V > 4 ? 4 : p.D % 2 == 0 && V > 2 ? 2 : 1);
+    for (s.lanes = 1; s.lanes < 32 && s.lanes * 2 <= items && s.lanes * s.samples * s.groups < kThreads;) s.lanes *= 2;
     s.by_words = divisor((uint32_t)s.words);
     s.by_width = divisor((uint32_t)s.width);
     s.by_D = divisor((uint32_t)p.D);
     s.by_S = divisor((uint32_t)p.S);
     s.by_groups = divisor((uint32_t)s.groups);
-    const size_t words = (size_t)s.rows * s.pitch, bytes = (words * V * esize + 15) / 16 * 16;
-    if (tensors == 1) s.shared = 2 * bytes + sizeof(float) * 2 * teams;
-    else s.shared = 4 * bytes + sizeof(float) * ((std::max(words * V, (size_t)half * s.width * 2) + 3) / 4 * 4 + (s.width + 3) / 4 * 4 + 6 * (size_t)teams);
-    if (s.shared > kMostShared || (long long)s.slabs * s.blocks > 0x7fffffffll) return false;
     *best = s;
     return true;
 }
 
-// Whether the groups of a sample are to be resident, and how: every slab width (multiples of the narrowest one that is whole
-// words, up to 512 bytes of a row), cluster size and block size that fits, against each other and against streaming.
-bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
+// Whether the groups of a sample are to be resident or packed, and how: every slab width (multiples of the narrowest one that is
+// whole words, up to 512 bytes of a row), cluster size and block size that fits, against each other and against streaming.
+bool search_plan(const Norm& p, int V, int esize, int tensors, Slab* best) {
     if (p.S > 1 << 20) return false;
     const int registers = tensors == 1 ? kResidentRegisters : kResidentBackwardRegisters;
     int unit = 1; // groups of the narrowest slab
     while ((unit * (long long)p.D) % V) ++unit;
     double least = streamed_time(p, V, esize, tensors);
     bool found = false;
-    Slab packed{};
-    if (pack(p, V, esize, tensors, unit, &packed)) {
-        if (const double time = packed_time(p, packed, V, esize, tensors); time < least) {
+    for (int cap = 32 * 1024 / tensors; cap >= 4 * 1024 / tensors; cap /= 2) {
+        Slab packed{};
+        if (!pack(p, V, esize, tensors, unit, cap, &packed)) continue;
+        if (const double time = packed_time(p, packed, V, tensors); time < least) {
             least = time;
             *best = packed;
             found = true;
@@ -1686,7 +1763,7 @@ bool search_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
 }
 
 // The search takes some ten microseconds; the last shapes of a thread are looked up instead.
-bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
+bool plan_of(const Norm& p, int V, int esize, int tensors, Slab* best) {
     struct Entry {
         long long S, C;
         int N, G, V, esize, tensors;
@@ -1705,7 +1782,7 @@ bool plan_resident(const Norm& p, int V, int esize, int tensors, Slab* best) {
     }
     Entry& e = entries[next++ % kEntries];
     e = Entry{p.S, p.C, p.N, p.G, V, esize, tensors, false, Slab{}};
-    e.fits = search_resident(p, V, esize, tensors, &e.slab);
+    e.fits = search_plan(p, V, esize, tensors, &e.slab);
     *best = e.slab;
     return e.fits;
 }
@@ -1721,7 +1798,7 @@ int word_elements(Norm& p, int dtype, uint64_t addresses) {
             if ((uint64_t)p.C * k * e % 16 || p.S % k || (uint64_t)p.C * k * e > 16ull * kThreads) continue;
             Slab s;
             const int V = a >= 4 ? 4 / e : 1;
-            if (plan_resident(p, V, e, 1, &s)) break; // short: better off in shared memory
+            if (plan_of(p, V, e, 1, &s)) break; // short: better off in shared memory
             p.fold = k;
             p.S /= k;
             p.C *= k;
@@ -1800,7 +1877,7 @@ size_t ring_bytes(size_t tile) {
 template <class T, int V>
 cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, void* workspace, cudaStream_t stream, int& launched) {
     Slab s;
-    const bool planned = p.fold == 1 && plan_resident(p, V, sizeof(T), 1, &s);
+    const bool planned = p.fold == 1 && plan_of(p, V, sizeof(T), 1, &s);
     if (planned && s.samples)
         return launch(sa_norm_packed_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream, launched, (T*)out,
                       (const T*)x, mean, rstd, s);
@@ -1825,11 +1902,12 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     auto join_params = [&](const float2* sums, int count, int C) {
         return launch(sa_norm_backward_params_kernel, (C + 31) / 32, 1024, 0, true, stream, launched, sums, dweight, dbias, count, C, p.param_dtype);
     };
-    const bool planned = p.fold == 1 && plan_resident(p, V, sizeof(T), 2, &s);
+    const bool planned = p.fold == 1 && plan_of(p, V, sizeof(T), 2, &s);
     if (planned && s.samples) {
-        float2* const sums = dweight || dbias ? (float2*)workspace : nullptr; // [blocks of a slab][C]
+        float2* const sums = s.blocks > 1 && (dweight || dbias) ? (float2*)workspace : nullptr; // [blocks of a slab][C]
         const cudaError_t e = launch(sa_norm_packed_backward_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream,
-                                     launched, (T*)dx, (const T*)dout, (const T*)x, mean, rstd, sums, s);
+                                     launched, (T*)dx, (const T*)dout, (const T*)x, mean, rstd, sums, s.blocks > 1 ? nullptr : dweight,
+                                     s.blocks > 1 ? nullptr : dbias, s);
         return e != cudaSuccess || !sums ? e : join_params(sums, s.blocks, (int)p.C);
     }
     if (planned) {
@@ -1889,9 +1967,10 @@ size_t sa_group_norm_workspace(const sideaware_group_norm_t& sh, bool backward) 
         const Norm p = describe(sh, nullptr, nullptr);
         Slab s;
         long long entries;
-        if (!plan_resident(p, V, e, backward ? 2 : 1, &s)) entries = streamed(p, V);
+        if (!plan_of(p, V, e, backward ? 2 : 1, &s)) entries = streamed(p, V);
         else if (!backward) entries = 0;
-        else entries = s.samples ? (long long)s.blocks * sh.C : sh.N > 1 ? (long long)sh.N * sh.C : 0;
+        else if (s.samples) entries = s.blocks > 1 ? (long long)s.blocks * sh.C : 0;
+        else entries = sh.N > 1 ? (long long)sh.N * sh.C : 0;
         if (entries > most) most = entries;
     }
     Norm p = describe(sh, nullptr, nullptr);

@@ -26,8 +26,8 @@
 //    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.2 us.
 //  * streamed: HBM.  2 x 262144 x 128 bf16: 74.5 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
 //    us for the copy-like second pass.
-//  * packed: instructions, about 280 of a warp for a word of each lane forward and 600 backward.  16384 x 1 x 2048 bf16: 48 us
-//    and 137 us (resident or streamed: 580 and 1080); 1 x 64 x 1280 bf16: 4.0 us, which is latency (resident 5.1).
+//  * packed: instructions, 190 of a warp for a word of each lane forward and 560 backward.  16384 x 1 x 2048 bf16: 45 us
+//    and 118 us (resident: 580 and 1080); 1 x 64 x 1280 bf16: 4.0 us, which is latency (resident 5.1).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1149,6 +1149,10 @@ sa_norm_resident_backward_kernel(T* dx, const T* dout, const T* x, const float* 
 // A block goes through tiles of `samples` whole samples of its slab; the next tile travels while one is worked on.  A thread
 // has one word of the row, so parameters and their gradients stay in its registers; `lanes` neighbouring threads take the
 // statistics of a group of a sample: its mean about one of its elements, then the squared deviations from that.
+// Blocks of an SM: what the registers allow without spills; forward four of whole words were slower than three with larger tiles
+// (65536 x 4 x 64 bf16: 30.9 against 24.2 us).
+constexpr int packed_on_sm(int tensors, bool whole) { return tensors == 1 || whole ? 3 : 2; }
+
 struct Pack {
     int slab, first_tile;
     int word, row_lane;
@@ -1181,11 +1185,13 @@ __device__ __forceinline__ Pack pack_of(const Slab& s) {
 // Rows of a tile (they follow one another in memory, whole samples).
 __device__ __forceinline__ int tile_samples(const Slab& s, int tile) { return min(s.samples, s.p.N - tile * s.samples); }
 
-// The values of this thread's channels out of one for each group, as pairs.  Which way is the same for all threads: words inside
-// groups, words with at most one border between pairs, or any.
-template <int V>
+// WHOLE in these kernels: groups are whole words, which takes a register instead of a word of them for every group's value
+// (16384 x 1 x 2048 bf16 backward: 137 us without it).
+// The values of this thread's channels out of one for each group, as pairs.  Otherwise words have at most one border between
+// pairs, or any, the same for all threads.
+template <int V, bool WHOLE>
 __device__ __forceinline__ void of_groups(const Pack& w, int D, const float* at, F2 (&out)[(V + 1) / 2]) {
-    if (D % V == 0) {
+    if (WHOLE) {
         const float v = at[w.g];
 #pragma unroll
         for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(v, v);
@@ -1214,9 +1220,9 @@ __device__ __forceinline__ void of_groups(const Pack& w, int D, const float* at,
 
 // Elements of an item, what a thread takes of a group at a time: as many as divide the group, up to a word.
 // f(std::integral_constant) for that number, the same for all threads.
-template <int V, class F>
+template <int V, bool WHOLE, class F>
 __device__ __forceinline__ void with_items(int D, F&& f) {
-    if (D % V == 0) f(std::integral_constant<int, V>());
+    if constexpr (WHOLE) f(std::integral_constant<int, V>());
     else if (V > 4 && D % 4 == 0) f(std::integral_constant<int, (V > 4 ? 4 : V)>());
     else if (V > 2 && D % 2 == 0) f(std::integral_constant<int, (V > 2 ? 2 : V)>());
     else f(std::integral_constant<int, 1>());
@@ -1252,8 +1258,8 @@ __device__ __forceinline__ void for_teams(const Slab& s, int samples, F&& f) {
     }
 }
 
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads, 3)
+template <class T, int V, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, packed_on_sm(1, WHOLE))
 sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __restrict__ rstd, const __grid_constant__ Slab s) {
     constexpr int P = (V + 1) / 2;
     using Word = SaVec<T, V>;
@@ -1293,7 +1299,7 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
             const int sub = threadIdx.x & (s.lanes - 1), count = real ? S * D : 0;
             const float k0 = real ? sa_to_float(*at) : 0.0f;
             float m = 0.0f, m2 = 0.0f;
-            with_items<V>(D, [&](auto size) {
+            with_items<V, WHOLE>(D, [&](auto size) {
                 constexpr int W = size.value;
                 auto each = [&](float about, auto&& f) {
                     const F2 c = f2(-about, -about);
@@ -1350,8 +1356,8 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
                 Word v = *row;
                 if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) { // the next sample
                     have = of;
-                    of_groups<V>(w, D, centre + of, m);
-                    of_groups<V>(w, D, scale + of, a);
+                    of_groups<V, WHOLE>(w, D, centre + of, m);
+                    of_groups<V, WHOLE>(w, D, scale + of, a);
 #pragma unroll
                     for (int k = 0; k < P; ++k) {
                         m[k] = negative(m[k]);
@@ -1369,8 +1375,8 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
 // `partial`: [blocks of a slab][C], each block's sums of (dz, dz u) over its samples; NULL: there is one block, dweight and
 // dbias are written here.  dz is kept in fp32 in
 // shared memory, so that the activation's derivative is worked out once.
-template <class T, int V>
-__global__ void __launch_bounds__(kThreads, 2)
+template <class T, int V, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, packed_on_sm(2, WHOLE))
 sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __restrict__ mean, const float* __restrict__ rstd,
                                float2* __restrict__ partial, void* __restrict__ dweight, void* __restrict__ dbias,
                                const __grid_constant__ Slab s) {
@@ -1444,8 +1450,8 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
                     const Word v = data[at], d = grad[at];
                     if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) { // the next sample
                         have = of;
-                        of_groups<V>(w, D, centre + of, m);
-                        of_groups<V>(w, D, scale + of, rs);
+                        of_groups<V, WHOLE>(w, D, centre + of, m);
+                        of_groups<V, WHOLE>(w, D, scale + of, rs);
                     }
                     F2 weight[P], bias[P];
                     shared_pairs<V>(weight, weights + w.word * V);
@@ -1477,7 +1483,7 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
             const float *const dz = flow + from, *const wg = weights + g * D;
             const float m = real ? centre[t] : 0.0f, rs = real ? scale[t] : 0.0f;
             float t1 = 0.0f, t2 = 0.0f;
-            with_items<V>(D, [&](auto size) {
+            with_items<V, WHOLE>(D, [&](auto size) {
                 constexpr int W = size.value;
                 constexpr int kPiece = W >= 4 ? 4 : W;
                 F2 s1 = f2(0.0f, 0.0f), s2 = s1;
@@ -1526,10 +1532,10 @@ sa_norm_packed_backward_kernel(T* dx, const T* dout, const T* x, const float* __
                 have = of;
                 F2 weight[P];
                 shared_pairs<V>(weight, weights + w.word * V);
-                of_groups<V>(w, D, centre + of, m);
-                of_groups<V>(w, D, scale + of, a);
-                of_groups<V>(w, D, first + of, m1);
-                of_groups<V>(w, D, second + of, m2);
+                of_groups<V, WHOLE>(w, D, centre + of, m);
+                of_groups<V, WHOLE>(w, D, scale + of, a);
+                of_groups<V, WHOLE>(w, D, first + of, m1);
+                of_groups<V, WHOLE>(w, D, second + of, m2);
 #pragma unroll
                 for (int k = 0; k < P; ++k) a[k] = a[k] * weight[k];
             }
@@ -1641,15 +1647,12 @@ double resident_time(const Norm& p, const Slab& s, int V, int esize, int tensors
     return fixed + rounds * (memory + arithmetic) + (rounds - 1.0) * 6.0;
 }
 
-// Blocks of the packed kernels that their registers let an SM have.
-int packed_on_sm(int tensors) { return tensors == 1 ? 3 : 2; }
-
 // The same for tiles of short samples: instructions, of the SM with the most tiles or of a block alone (fitted to 20 shapes, with
-// 1,000 to 134 million elements; the choice took at most 5 % longer than the better way).
+// 1,000 to 34 million elements; the choice took at most 9 % longer than the better way).
 double packed_time(const Norm& p, const Slab& s, int V, int tensors) {
     const double each = std::ceil((double)s.tiles / s.blocks), on_sm = std::ceil((double)s.slabs * s.blocks / 148);
     const double thousands = s.rows * s.width * 1e-3 * (V == 8 ? 1.0 : V == 4 ? 1.7 : 2.4) * (p.D % V ? 1.3 : 1.0);
-    const double most = std::min(on_sm, (double)packed_on_sm(tensors)), rounds = std::ceil(on_sm / most);
+    const double most = std::min(on_sm, (double)packed_on_sm(tensors, p.D % V == 0)), rounds = std::ceil(on_sm / most);
     if (tensors == 1) return 3.0 + rounds * each * (0.4 + thousands * std::max(0.3, 0.18 * most));
     return 5.6 + rounds * each * (0.7 + thousands * std::max(0.5, 0.38 * most));
 }
@@ -1680,8 +1683,8 @@ bool pack(const Norm& p, int V, int esize, int tensors, int unit, int cap, Slab*
     s.threads = kThreads;
     s.row_lanes = kThreads / s.words;
     s.parts = shares((s.row_lanes + 1) / 2, kThreads / s.width);
-    const int on_sm = packed_on_sm(tensors);
-    const size_t most = tensors == 1 ? 75 * 1024 : 113 * 1024; // for three and two blocks
+    const int on_sm = packed_on_sm(tensors, p.D % V == 0);
+    const size_t most = (228 / on_sm - 1) * 1024;
     s.samples = (int)std::max(1ll, std::min({cap / (column * groups), (long long)p.N, (long long)p.N * s.slabs / (148 * on_sm)}));
     for (;; --s.samples) {
         const size_t words = (size_t)s.samples * p.S * s.pitch, bytes = (words * V * esize + 15) / 16 * 16, teams = (size_t)s.samples * s.groups;
@@ -1879,7 +1882,7 @@ cudaError_t forward(void* out, float* mean, float* rstd, const void* x, Norm p, 
     Slab s;
     const bool planned = p.fold == 1 && plan_of(p, V, sizeof(T), 1, &s);
     if (planned && s.samples)
-        return launch(sa_norm_packed_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream, launched, (T*)out,
+        return launch(p.D % V == 0 ? sa_norm_packed_kernel<T, V, true> : sa_norm_packed_kernel<T, V, V == 1>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream, launched, (T*)out,
                       (const T*)x, mean, rstd, s);
     if (planned)
         return launch_clusters(sa_norm_resident_kernel<T, V>, s, stream, launched, (T*)out, (const T*)x, mean, rstd, s);
@@ -1905,7 +1908,7 @@ cudaError_t backward(void* dx, void* dweight, void* dbias, const void* dout, con
     const bool planned = p.fold == 1 && plan_of(p, V, sizeof(T), 2, &s);
     if (planned && s.samples) {
         float2* const sums = s.blocks > 1 && (dweight || dbias) ? (float2*)workspace : nullptr; // [blocks of a slab][C]
-        const cudaError_t e = launch(sa_norm_packed_backward_kernel<T, V>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream,
+        const cudaError_t e = launch(p.D % V == 0 ? sa_norm_packed_backward_kernel<T, V, true> : sa_norm_packed_backward_kernel<T, V, V == 1>, (long long)s.slabs * s.blocks, kThreads, s.shared, false, stream,
                                      launched, (T*)dx, (const T*)dout, (const T*)x, mean, rstd, sums, s.blocks > 1 ? nullptr : dweight,
                                      s.blocks > 1 ? nullptr : dbias, s);
         return e != cudaSuccess || !sums ? e : join_params(sums, s.blocks, (int)p.C);

@@ -297,7 +297,8 @@ class SideAware:
         arrangement "own": every axis has a run of pairs and frequencies theta^(-j/n) of its own; "shared": one series
         theta^(-i/pairs), each axis a run of it; "interleaved": the same series, its pairs dealt to the axes in turn."""
         import torch
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = torch.device("cuda" if device is None else device)
+        assert device.type == "cuda", f"the spectrum is made on a CUDA device, not on {device}"
         index = torch.cuda.current_device() if device.index is None else device.index
         assert arrangement in _ROPE_ARRANGEMENTS, f"arrangement must be one of {sorted(_ROPE_ARRANGEMENTS)}"
         pairs = [int(n) for n in pairs_per_axis]

@@ -177,3 +177,10 @@ def test_python_wrappers_refuse_cpu_tensors(sa):
         sa.group_norm_forward(x, x, x, x, None, None, 2)
     with pytest.raises(AssertionError, match="CUDA"):
         sa.rope_axes_forward(torch.zeros(1, 2, 3, 8), torch.zeros(1, 1, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int64), 1, 1)
+
+
+@pytest.mark.parametrize("device", ["cpu", torch.device("cpu", 0), "meta"])
+def test_rope_axes_spectrum_refuses_devices_that_are_not_cuda(sa, device):
+    """Refused before anything is allocated or launched: the kernel would write through a host address."""
+    with pytest.raises(AssertionError, match="CUDA"):
+        sa.rope_axes_spectrum((4, 4), device=device)

@@ -253,10 +253,11 @@ class SideAware:
     def rope_precompute_freqs(self, dim: int, end: int, theta: float = 10000.0, use_scaled: bool = False, device=None):
         """The fp32 table [end, dim/2, 2] of (cos, sin) that rope_forward / rope_backward read, made on the GPU."""
         import torch
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = torch.device("cuda" if device is None else device)
+        assert device.type == "cuda", f"the table is made on a CUDA device, not on {device}"
         table = torch.empty((end, dim // 2, 2), dtype=torch.float32, device=device)
-        self.rope_precompute_freqs_ptr(table.data_ptr(), dim, end, float(theta), use_scaled, device.index,
-                                       torch.cuda.current_stream(device))
+        self.rope_precompute_freqs_ptr(table.data_ptr(), dim, end, float(theta), use_scaled, table.device.index,
+                                       torch.cuda.current_stream(table.device))
         return table
 
     def silu_mul(self, out, a, b, scale: float) -> None:

@@ -312,9 +312,11 @@ class SideAware:
 
     def _rope_axes(self, call, what, qkv, positions, spectrum, n_q_heads, n_kv_heads, layout) -> None:
         import torch
+        B, T, H, HS = qkv.shape
+        # the C ABI has 32-bit sizes, and ctypes would cut off what does not fit; negative ones are refused as well
+        assert (B | T | H | HS | n_q_heads | n_kv_heads | spectrum.numel() | positions.shape[0]) >> 31 == 0, "sizes must be below 2^31"
         device = qkv.get_device()
         assert device >= 0 and positions.get_device() == device and spectrum.get_device() == device, "all tensors must be on one CUDA device"
-        B, T, H, HS = qkv.shape
         assert H == n_q_heads + 2 * n_kv_heads, "head dimension must hold q, k and v heads"
         sb, st, sh, se = qkv.stride()
         assert (se == 1 or HS == 1) and (sh == HS or H <= 1), "heads and their elements must be dense"
@@ -345,10 +347,12 @@ class SideAware:
         """Checks what forward and backward share; returns (shape for the C ABI, workspace, its size).  `like`: tensors shaped
         as x; `stats`: fp32 [N, groups]; `params`: tensors of C entries, or None."""
         import torch
-        device = x.get_device()
-        assert device >= 0 and x.is_contiguous() and x.dim() >= 2, "x must be a dense CUDA tensor [N, ..., C]"
-        size, dtype = x.shape, x.dtype
+        size, dtype, device = x.shape, x.dtype, x.get_device()
+        assert len(size) >= 2, "x must be a dense CUDA tensor [N, ..., C]"
         N, C = size[0], size[-1]
+        # the C ABI has 32-bit sizes (S: 64 bits), and ctypes would cut off what does not fit
+        assert (N | C | groups) >> 31 == 0, "samples, channels and groups must be below 2^31"
+        assert device >= 0 and x.is_contiguous(), "x must be a dense CUDA tensor [N, ..., C]"
         for t in like:
             assert t.shape == size and t.dtype is dtype and t.is_contiguous() and t.get_device() == device, \
                 "out, dx and dout must be dense tensors of x's shape, dtype and device"

@@ -33,6 +33,11 @@ def _dtype_code(dtype) -> int:
     return code
 
 
+def _below_2_31(*sizes) -> None:
+    """The C ABI has 32-bit sizes, and ctypes would cut off what does not fit."""
+    assert all(-2 ** 31 <= n < 2 ** 31 for n in sizes), "sizes must be below 2^31"
+
+
 def _stream_ptr(stream) -> int:
     if stream is None:
         return 0
@@ -119,17 +124,20 @@ class SideAware:
         self._checked(before, "sideaware_memcpy")
 
     def rope_backward_ptr(self, dqkv: int, freqs: int, B, T, Nq, Nkv, HS, bf16: bool, device: int = 0, stream=None) -> None:
+        _below_2_31(B, T, Nq, Nkv, HS)
         rc = self.lib.sideaware_rope_backward(dqkv, freqs, B, T, Nq, Nkv, HS, 1 if bf16 else 0, device, _stream_ptr(stream))
         if rc != 0:
             raise RuntimeError(f"sideaware_rope_backward failed with CUDA error {rc}: {self.last_error()}")
 
     def rope_forward_ptr(self, qkv: int, freqs: int, B, T, Nq, Nkv, HS, bf16: bool, device: int = 0, stream=None) -> None:
+        _below_2_31(B, T, Nq, Nkv, HS)
         rc = self.lib.sideaware_rope_forward(qkv, freqs, B, T, Nq, Nkv, HS, 1 if bf16 else 0, device, _stream_ptr(stream))
         if rc != 0:
             raise RuntimeError(f"sideaware_rope_forward failed with CUDA error {rc}: {self.last_error()}")
 
     def rope_precompute_freqs_ptr(self, table: int, dim: int, end: int, theta: float, use_scaled: bool,
                                   device: int = 0, stream=None) -> None:
+        _below_2_31(dim, end)
         rc = self.lib.sideaware_rope_precompute_freqs(table, dim, end, theta, 1 if use_scaled else 0, device, _stream_ptr(stream))
         if rc != 0:
             raise RuntimeError(f"sideaware_rope_precompute_freqs failed with CUDA error {rc}: {self.last_error()}")

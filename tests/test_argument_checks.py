@@ -44,3 +44,21 @@ def test_group_norm_refuses_sizes_past_31_bits(sa, shape, groups):
         sa.group_norm_forward(x, stats, stats, x, None, None, groups)
     with pytest.raises(AssertionError, match="2.31"):
         sa.group_norm_backward(x, None, None, x, x, stats, stats, None, None, groups)
+
+
+P = 1 << 20  # an address that is never read: every call here is refused on the host
+
+
+@pytest.mark.parametrize("place", range(5))
+@pytest.mark.parametrize("name", ["rope_forward_ptr", "rope_backward_ptr"])
+def test_rope_refuses_sizes_past_31_bits(sa, name, place):
+    sizes = [2, 3, 4, 2, 16]
+    sizes[place] += 2 ** 32
+    with pytest.raises(AssertionError, match="2.31"):
+        getattr(sa, name)(P, P, *sizes, True)
+
+
+@pytest.mark.parametrize("sizes", [(2 ** 32 + 64, 16), (64, 2 ** 32 + 16)])
+def test_rope_precompute_freqs_refuses_sizes_past_31_bits(sa, sizes):
+    with pytest.raises(AssertionError, match="2.31"):
+        sa.rope_precompute_freqs_ptr(P, *sizes, 10000.0, False)

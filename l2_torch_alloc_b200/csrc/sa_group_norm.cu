@@ -22,7 +22,7 @@
 // Bound and measured on a B200 (device time of a call, three sets of inputs in turn):
 //  * resident: the phases of a block follow one another, and each moves about 4 TB/s alone.  8 x 4096 x 320 bf16: 16.7 us (6.4
 //    at the copy's rate), of 31,000 cycles 12,000 are for the rows to arrive, 5,000 for the statistics to go around and
-//    11,500 for SiLU and the stores (without SiLU: 1.4 us less).  Backward the activation's derivative is worked out twice, 24
+//    11,500 for SiLU and the stores (without SiLU: 1.4 us less).  Backward the activation's derivative is worked out twice, 32
 //    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.2 us.
 //  * streamed: HBM.  2 x 262144 x 128 bf16: 74.5 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
 //    us for the copy-like second pass.
@@ -71,13 +71,6 @@ __device__ __forceinline__ void join(Moments& a, const Moments& b) {
     a.mean = fmaf(d, f, a.mean);
     a.m2 += b.m2 + d * d * a.n * f;
     a.n = n;
-}
-
-// sigmoid: fp32 storage wants all of fp32, for 16-bit storage the fast forms' 2^-21 is far below a rounding
-template <class T>
-__device__ __forceinline__ float sigmoid(float z) {
-    if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
-    return __fdividef(1.0f, 1.0f + __expf(-z));
 }
 
 // ---------------------------------------------------------------------------
@@ -175,25 +168,31 @@ __device__ __forceinline__ void shared_pairs(F2 (&out)[(V + 1) / 2], const float
     for (int k = 0; k < (V + 1) / 2; ++k) out[k] = f2(p[2 * k], 2 * k + 1 < V ? p[2 * k + 1] : 0.0f);
 }
 
-// 16-bit storage: one reciprocal for both, 1 / a = b / (a b).  The special-function unit is what an activation waits for (8
-// cycles a warp and operation), so 1.5 of them for each element instead of 2.  The exponent is held below 60 so that a b stays
-// finite: sigmoid is off by less than 1e-18 beyond that.
+// The activation of a word's pairs.  fp32 storage wants all of fp32.  16-bit storage takes the fast exponential and reciprocal, whose
+// 2^-22 (and a rounding of the exponent) are far below a rounding of the result; below z = -87 sigmoid is 0, and z sigmoid(z)
+// and the derivative with it, which are under 2^-119 there.
+__device__ __forceinline__ float exp2_fast(float v) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v));
+    return v;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
+    return v;
+}
+// 1 + exp(-z)
+__device__ __forceinline__ void denominators(F2 z, float& a, float& b) {
+    split(z * f2(-1.44269504f, -1.44269504f), a, b); // -log2 e
+    split(f2(exp2_fast(a), exp2_fast(b)) + f2(1.0f, 1.0f), a, b);
+}
 template <class T>
 __device__ __forceinline__ F2 sigmoid2(F2 z) {
-    float x, y;
+    float a, b;
     if constexpr (sizeof(T) == 4) {
-        split(z, x, y);
-        return f2(sigmoid<T>(x), sigmoid<T>(y));
+        split(z, a, b);
+        return f2(1.0f / (1.0f + expf(-a)), 1.0f / (1.0f + expf(-b)));
     }
-    split(z * f2(-1.44269504f, -1.44269504f), x, y); // -log2 e
-    x = fminf(x, 60.0f);
-    y = fminf(y, 60.0f);
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
-    split(f2(x, y) + f2(1.0f, 1.0f), x, y);
-    float r = x * y;
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
-    return f2(r, r) * f2(y, x);
+    denominators(z, a, b);
+    return f2(reciprocal_fast(a), reciprocal_fast(b));
 }
 
 // The inner loops exist with and without the activation, which is one branch around them: with_activation(silu, f) calls
@@ -204,13 +203,45 @@ __device__ __forceinline__ void with_activation(int silu, F&& f) {
     else f(std::false_type{});
 }
 
-template <class T, bool SILU>
-__device__ __forceinline__ F2 activation2(F2 z) {
-    if constexpr (!SILU) return z;
-    return z * sigmoid2<T>(z);
+// use(k, activation of z(k)) for the P pairs of a word, possibly a second time.  16-bit storage: the special-function unit is what
+// an activation waits for (8 cycles a warp and operation), so a pair has one reciprocal, 1 / a = b / (a b), 1.5 operations for each
+// element instead of 2.  Where a b is no number any more (from z = -43 on) or a NaN, which its neighbour must not see, the word is
+// done again with one for each element.  (The smallest of the reciprocals tells; a test of z before them took 1 to 5 % of a call,
+// limits on z 1 to 4 %, a reciprocal for each element always 3 to 12 %.)
+template <class T, bool SILU, int P, class Z, class Use>
+__device__ __forceinline__ void activation(Z&& z, Use&& use) {
+    if constexpr (!SILU) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) use(k, z(k));
+    } else if constexpr (sizeof(T) == 4 || P == 1) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            const F2 v = z(k);
+            use(k, v * sigmoid2<T>(v));
+        }
+    } else {
+        float least = 1.0f;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            float a, b;
+            const F2 v = z(k);
+            denominators(v, a, b);
+            const float r = reciprocal_fast(a * b);
+            asm("min.NaN.f32 %0, %0, %1;" : "+f"(least) : "f"(r));
+            use(k, v * (f2(r, r) * f2(b, a)));
+        }
+        if (__builtin_expect(!(least > 0.0f), 0)) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const F2 v = z(k);
+                use(k, v * sigmoid2<T>(v));
+            }
+        }
+    }
 }
 
-// dy act'(z) = dy s (1 + z (1 - s))
+// dy act'(z) = dy s (1 + z (1 - s)).  A reciprocal for each element: 1 - s is exactly 0 for large z then.  (One for a pair, and
+// 1 - s = exp(-z) s: no faster.)
 template <class T, bool SILU>
 __device__ __forceinline__ F2 through_activation2(F2 dy, F2 z) {
     if constexpr (!SILU) return dy;
@@ -610,10 +641,10 @@ sa_norm_apply_kernel(T* out, const T* x, const float* __restrict__ mean, const f
         stream_rows<kRingWords / kStreamStages>(
             w.rows, [&](int slot) { in.fetch(slot); }, [](int, int) {},
             [&](int slot) {
-                SaVec<T, V> v = in.row(slot);
-#pragma unroll
-                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], b[k])));
-                sa_store_stream<T, V>(to, v);
+                const SaVec<T, V> v = in.row(slot);
+                SaVec<T, V> y;
+                activation<T, silu.value, P>([&](int k) { return fma2(pair_of(v, k) + m[k], a[k], b[k]); }, [&](int k, F2 e) { set_pair(y, k, e); });
+                sa_store_stream<T, V>(to, y);
                 to -= step;
             });
     });
@@ -971,10 +1002,10 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
             const SaVec<T, V>* row = mine;
 #pragma unroll 2
             for (int u = 0; u < w.rows; ++u, to += step, row += stride) {
-                SaVec<T, V> v = *row;
-#pragma unroll
-                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], b[k])));
-                sa_store<T, V>(to, v);
+                const SaVec<T, V> v = *row;
+                SaVec<T, V> y;
+                activation<T, silu.value, P>([&](int k) { return fma2(pair_of(v, k) + m[k], a[k], b[k]); }, [&](int k, F2 e) { set_pair(y, k, e); });
+                sa_store<T, V>(to, y);
             }
         });
     }
@@ -1353,7 +1384,7 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
         int have = -1;
         with_activation(p.silu, [&](auto silu) {
             for (int r = w.row_lane; r < rows; r += s.row_lanes, to += step, row += stride) {
-                Word v = *row;
+                const Word v = *row;
                 if (const int of = (int)s.by_S.div((uint32_t)r) * s.groups; of != have) { // the next sample
                     have = of;
                     of_groups<V, WHOLE>(w, D, centre + of, m);
@@ -1364,9 +1395,9 @@ sa_norm_packed_kernel(T* out, const T* x, float* __restrict__ mean, float* __res
                         a[k] = a[k] * weight[k];
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < P; ++k) set_pair(v, k, activation2<T, silu.value>(fma2(pair_of(v, k) + m[k], a[k], bias[k])));
-                sa_store_stream<T, V>(to, v);
+                Word y;
+                activation<T, silu.value, P>([&](int k) { return fma2(pair_of(v, k) + m[k], a[k], bias[k]); }, [&](int k, F2 e) { set_pair(y, k, e); });
+                sa_store_stream<T, V>(to, y);
             }
         });
     }

@@ -316,6 +316,7 @@ class SideAware:
         self._done(self.lib.sideaware_rope_axes_spectrum(
             spectrum.data_ptr(), (ctypes.c_int * len(pairs))(*pairs), len(pairs), float(theta), _ROPE_ARRANGEMENTS[arrangement],
             index, _current_stream(index)), "sideaware_rope_axes_spectrum")
+        spectrum.rope_axes = len(pairs)  # what the positions are checked against; a copy of the tensor goes without
         return spectrum
 
     def _rope_axes(self, call, what, qkv, positions, spectrum, n_q_heads, n_kv_heads, layout) -> None:
@@ -323,12 +324,13 @@ class SideAware:
         B, T, H, HS = qkv.shape
         # the C ABI has 32-bit sizes, and ctypes would cut off what does not fit; negative ones are refused as well
         assert (B | T | H | HS | n_q_heads | n_kv_heads | spectrum.numel() | positions.shape[0]) >> 31 == 0, "sizes must be below 2^31"
+        axes = positions.shape[0]
+        assert getattr(spectrum, "rope_axes", axes) == axes, "positions must have the axes that the spectrum was made with"
         device = qkv.get_device()
         assert device >= 0 and positions.get_device() == device and spectrum.get_device() == device, "all tensors must be on one CUDA device"
         assert H == n_q_heads + 2 * n_kv_heads, "head dimension must hold q, k and v heads"
         sb, st, sh, se = qkv.stride()
         assert (se == 1 or HS == 1) and (sh == HS or H <= 1), "heads and their elements must be dense"
-        axes = positions.shape[0]
         assert positions.dim() == 3 and tuple(positions.shape[1:]) == (B, T), "positions must be [axes, B, T]"
         assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
         assert spectrum.dim() == 1 and spectrum.dtype == torch.int64 and spectrum.is_contiguous(), "spectrum must be int64 [pairs]"
@@ -340,7 +342,8 @@ class SideAware:
     def rope_axes_forward(self, qkv, positions, spectrum, n_q_heads: int, n_kv_heads: int, layout: str = "interleaved") -> None:
         """Rotary positions with several axes, in place on packed [B, T, Nq + 2 Nkv, HS] (fp32, bf16 or fp16; any strides
         over B and T): pair i of every q and k head turns by positions[axis of i, b, t] times its frequency.
-        positions: int32 or int64 [axes, B, T], any strides and values, with the spectrum's axes; spectrum:
+        positions: int32 or int64 [axes, B, T], any strides and values, with the spectrum's axes (others are refused; where
+        the spectrum is a copy that no longer knows them, pairs of axes that the positions lack, and neighbours, become NaN); spectrum:
         rope_axes_spectrum.  A head of which the spectrum's pairs fill only a part keeps its remaining elements.  layout:
         pair i = elements (2i, 2i + 1) ("interleaved") or (i, i + pairs) ("halves")."""
         self._rope_axes(self.lib.sideaware_rope_axes_forward, "sideaware_rope_axes_forward", qkv, positions, spectrum,

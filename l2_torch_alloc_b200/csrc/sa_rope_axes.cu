@@ -113,21 +113,26 @@ sa_rope_axes_kernel(T* __restrict__ x, const void* __restrict__ positions, const
     float c[kPairs], s[kPairs];
     const long long place = b * sh.pos_stride_b + t * sh.pos_stride_t;
     uint32_t have = 0xffffffffu; // neighbouring pairs mostly share their axis
+    bool lacking = false;
     long long pos = 0;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
         const unsigned long long f = __ldg(spectrum + slot * kPairs + i);
-        const uint32_t axis = min((uint32_t)f & 7u, sh.axes - 1u);
+        const uint32_t axis = (uint32_t)f & 7u;
         if (axis != have) {
-            const long long at = place + axis * sh.pos_stride_axis;
+            lacking |= axis >= sh.axes;
+            const long long at = place + (axis < sh.axes ? axis : 0u) * sh.pos_stride_axis;
             pos = sh.wide_positions ? __ldg(static_cast<const long long*>(positions) + at)
                                     : (long long)__ldg(static_cast<const int*>(positions) + at);
             have = axis;
         }
         const unsigned long long product = (unsigned long long)pos * (f & ~7ull);
         cos_sin_of_turn((uint32_t)(product >> 32), c[i], s[i]);
-        if (sh.inverse) s[i] = -s[i];
     }
+    // a spectrum of other positions: no number rather than a wrong one
+    const float direction = lacking ? __int_as_float(0x7fffffff) : sh.inverse ? -1.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) s[i] *= direction;
     if constexpr (HALVES && V > 1) { // two neighbouring pairs of a head at a time
 #pragma unroll
         for (int u = 0; u < U; ++u) {

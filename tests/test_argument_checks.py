@@ -62,3 +62,13 @@ def test_rope_refuses_sizes_past_31_bits(sa, name, place):
 def test_rope_precompute_freqs_refuses_sizes_past_31_bits(sa, sizes):
     with pytest.raises(AssertionError, match="2.31"):
         sa.rope_precompute_freqs_ptr(P, *sizes, 10000.0, False)
+
+
+@pytest.mark.parametrize("made, axes", [(3, 2), (2, 3), (1, 2)])
+@pytest.mark.parametrize("name", ["rope_axes_forward", "rope_axes_backward"])
+def test_rope_axes_refuses_positions_of_other_axes(sa, name, made, axes):
+    """A spectrum knows how many axes it was made with (rope_axes_spectrum sets that)."""
+    spectrum = torch.zeros(8, dtype=torch.int64)
+    spectrum.rope_axes = made
+    with pytest.raises(AssertionError, match="axes"):
+        getattr(sa, name)(torch.zeros(2, 3, 8, 16), torch.zeros(axes, 2, 3, dtype=torch.int32), spectrum, 4, 2)

@@ -1,0 +1,40 @@
+"""Rotary positions with several axes: calls whose arguments do not fit one another, and the largest rows."""
+import pytest
+import torch
+
+from tests import image_operator_reference as ref
+from tests.test_gpu_image_operators import BF16, F16, F32, close, randn, sa  # noqa: F401 (sa: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def test_positions_of_other_axes_are_refused(sa):
+    x, spectrum = randn(2, 3, 8, 16, seed=1), sa.rope_axes_spectrum((2, 3, 3))
+    before = x.clone()
+    for axes in (1, 2, 4):
+        places = torch.ones(axes, 2, 3, dtype=torch.int32, device="cuda")
+        for call in (sa.rope_axes_forward, sa.rope_axes_backward):
+            with pytest.raises(AssertionError, match="axes"):
+                call(x, places, spectrum, 4, 2)
+    assert torch.equal(x, before)
+    sa.rope_axes_forward(x, torch.ones(3, 2, 3, dtype=torch.int32, device="cuda"), spectrum, 4, 2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("layout", ["interleaved", "halves"])
+def test_axes_that_the_positions_lack_become_nan(sa, layout, dtype):
+    """A copy of the spectrum no longer knows its axes: the kernel sees them in its entries.  Every other element is NaN with them
+    (a thread has several pairs) or right; what is not turned stays."""
+    B, T, q, kv, pairs = 2, 5, 3, 2, (3, 6, 7)
+    for head, arrangement in ((32, "own"), (40, "interleaved")):
+        x = randn(B, T, q + 2 * kv, head, seed=3, dtype=dtype)
+        before = x.clone()
+        places = torch.randint(0, 500, (3, B, T), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+        sa.rope_axes_forward(x, places[:2], sa.rope_axes_spectrum(pairs, arrangement=arrangement).clone(), q, kv, layout)
+        want, bound = ref.rope(before.double(), places, pairs, 10000.0, arrangement, q, kv, layout)
+        lacking = torch.tensor([i for i, (_, a) in enumerate(ref.frequencies(pairs, 10000.0, arrangement)) if a == 2], device="cuda")
+        elements = torch.cat((2 * lacking, 2 * lacking + 1) if layout == "interleaved" else (lacking, lacking + sum(pairs)))
+        assert torch.isnan(x[:, :, :q + kv, elements]).all()
+        assert not torch.isnan(x[:, :, q + kv:]).any() and not torch.isnan(x[..., 2 * sum(pairs):]).any()
+        want[torch.isnan(x)] = float("nan")
+        close(x, want, bound)

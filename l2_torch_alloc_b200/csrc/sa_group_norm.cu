@@ -65,8 +65,11 @@ struct Moments {
 };
 
 __device__ __forceinline__ void join(Moments& a, const Moments& b) {
+    if (a.n == 0.0f) { // b as it is: a weight of nearly 1 would move a mean far from zero by more than the deviations
+        a = b;
+        return;
+    }
     const float n = a.n + b.n;
-    if (n == 0.0f) return;
     const float d = b.mean - a.mean, f = __fdividef(b.n, n); // a weight: two roundings more do no harm
     a.mean = fmaf(d, f, a.mean);
     a.m2 += b.m2 + d * d * a.n * f;
@@ -472,6 +475,8 @@ __device__ __forceinline__ void for_groups(int g0, int g1, int lanes, F&& f) {
         f(min(mine, g1), mine <= g1);
     }
 }
+// Place of the first channel of group g in a slab.
+__device__ __forceinline__ int first_place(const Norm& p, long long first, int g) { return (int)max((long long)g * p.D - first, 0ll); }
 // f(j) for this lane's share of the places j of group g in a slab
 template <class F>
 __device__ __forceinline__ void for_group(const Norm& p, long long first, int channels, int g, int lanes, F&& f) {
@@ -502,7 +507,7 @@ sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, co
 #pragma unroll
     for (int k = 0; k < P; ++k) k0[k] = sum[k] = square[k] = m[k] = q[k] = f2(0.0f, 0.0f);
     auto fold = [&] {
-        const float c = (float)have, inv = 1.0f / c, share = __fdividef(c, n + c), weight = n * share;
+        const float c = (float)have, inv = 1.0f / c, share = n > 0.0f ? __fdividef(c, n + c) : 1.0f, weight = n * share;
 #pragma unroll
         for (int k = 0; k < P; ++k) {
             const F2 part = sum[k] * f2(inv, inv), d = part + negative(k0[k] + m[k]);
@@ -557,12 +562,13 @@ sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, co
     const int lanes = group_lanes(p);
     for_groups(g0, g1, lanes, [&](int g, bool is) {
         float n_channels = 0.0f, sum = 0.0f, m2 = 0.0f;
+        const float about = centre[first_place(p, w.first, g)]; // the mean of the group's first channel here: what is summed is small
         for_group(p, w.first, w.channels, g, lanes, [&](int j) {
             n_channels += 1.0f;
-            sum += centre[j];
+            sum += centre[j] - about;
             m2 += deviation[j];
         });
-        const float mg = __fdividef(lanes_sum(sum, lanes), lanes_sum(n_channels, lanes));
+        const float mg = about + __fdividef(lanes_sum(sum, lanes), lanes_sum(n_channels, lanes));
         for_group(p, w.first, w.channels, g, lanes, [&](int j) {
             const float off = centre[j] - mg;
             m2 = fmaf(off * off, (float)w.block_rows, m2);
@@ -955,15 +961,17 @@ sa_norm_resident_kernel(T* out, const T* x, float* __restrict__ mean, float* __r
     };
     for (int g = warp; g < w.groups; g += warps) {
         float sum = 0.0f, m2 = 0.0f;
+        const float about = centre[g * p.D]; // a mean of the group's first channel: what is summed is small
+        __syncwarp();                        // before it becomes that of all rows
         for (int d = lane; d < p.D; d += 32) { // a channel's mean and squared deviations
             const int c = g * p.D + d;
             const float2 t = channel_sum<V>(s, tile, c);
             const float off = t.x * rows_inv, mc = centre[c] + off;
             centre[c] = mc;
             m2 += fmaf(-t.x, off, t.y);
-            sum += mc;
+            sum += mc - about;
         }
-        const float mg = warp_sum(sum) * D_inv;
+        const float mg = about + warp_sum(sum) * D_inv;
         for (int d = lane; d < p.D; d += 32) {
             const float off = centre[g * p.D + d] - mg; // written by this lane
             m2 = fmaf(off * off, (float)w.block_rows, m2);

@@ -72,7 +72,7 @@ __device__ __forceinline__ void join(Moments& a, const Moments& b) {
     const float n = a.n + b.n;
     const float d = b.mean - a.mean, f = __fdividef(b.n, n); // a weight: two roundings more do no harm
     a.mean = fmaf(d, f, a.mean);
-    a.m2 += b.m2 + d * d * a.n * f;
+    a.m2 += b.m2 + d * (d * (a.n * f));
     a.n = n;
 }
 
@@ -512,7 +512,7 @@ sa_norm_partial_kernel(const T* __restrict__ x, float2* __restrict__ partial, co
         for (int k = 0; k < P; ++k) {
             const F2 part = sum[k] * f2(inv, inv), d = part + negative(k0[k] + m[k]);
             q[k] = q[k] + fma2(negative(sum[k]), part, square[k]);
-            q[k] = fma2(d * d, f2(weight, weight), q[k]);
+            q[k] = fma2(d * f2(weight, weight), d, q[k]); // weight first: 0 for the first rows, however far they are from zero
             m[k] = fma2(d, f2(share, share), m[k]);
             sum[k] = square[k] = f2(0.0f, 0.0f);
         }

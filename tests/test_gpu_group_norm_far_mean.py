@@ -42,3 +42,25 @@ def test_mean_far_from_zero(sa, shape, offset):
     spread = (g - exact[:, None, :, None]).abs().amax(dim=(1, 3))
     steps = 3 + (3 if S < 5000 else 10 + (S / 444 + 8) / 32)
     close(mean, exact, steps * U * exact.abs() + ref.CHAIN * spread)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_large_numbers(sa, shape):
+    """The square of a value is past fp32's range, that of a deviation is not."""
+    N, S, C, G = shape
+    x = torch.full((N, S, C), 1e30, device="cuda")
+    out, mean, rstd = norm_forward(sa, x, None, None, G, silu=False)
+    assert torch.equal(mean, x[:, 0, :1].expand(N, G)) and not out.any()
+    close(rstd, torch.full_like(rstd.double(), 1e-5).rsqrt(), 2 * U * rstd.double())
+    x = randn(N, S, C, seed=7) * 1e15 + 1e20
+    out, mean, rstd = norm_forward(sa, x, None, None, G, silu=False)
+    g = x.double().view(N, S, G, C // G)
+    exact = g.mean(dim=(1, 3))
+    deviation = g - exact[:, None, :, None]
+    error = (3 + (3 if S < 5000 else 10 + (S / 444 + 8) / 32)) * U * exact.abs() + ref.CHAIN * deviation.abs().amax(dim=(1, 3))
+    close(mean, exact, error)
+    if S * C // G > 1:  # every deviation is off by the error of what it is taken about, twice at most: the square by 2 e |d| + e^2
+        var = deviation.square().mean(dim=(1, 3))
+        off = 2 * error * deviation.abs().mean(dim=(1, 3)) + error.square() + ref.CHAIN * var
+        limit = (var - 2 * off).clamp(min=1e-30).rsqrt() - var.rsqrt()
+        close(rstd, var.rsqrt(), limit)

@@ -822,7 +822,8 @@ sa_norm_backward_apply_kernel(T* dx, const T* dout, const T* x, const float* __r
     const int lanes = s.slabs == 1 ? group_lanes(p) : 32;
     for_groups(first_group(p, w.first), last_group(p, w.first, w.channels), lanes, [&](int g, bool is) {
         float2 t = make_float2(0.0f, 0.0f);
-        for (int d = threadIdx.x & (lanes - 1); d < p.D; d += lanes) {
+        // (lanes without a group of their own leave the last one's channels alone: its own lanes overwrite them below)
+        for (int d = threadIdx.x & (lanes - 1); is && d < p.D; d += lanes) {
             const int c = g * p.D + d;
             const float2 e = s.slabs == 1 ? make_float2(first[c], second[c]) : weighted(c);
             t.x += e.x;

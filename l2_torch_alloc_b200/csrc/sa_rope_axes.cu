@@ -165,9 +165,8 @@ cudaError_t launch(void* qkv, const void* positions, const void* spectrum, Shape
     constexpr int U = V * (int)sizeof(T) == 16 && HALVES ? 2 : 4; // 64 bytes of each thread are in flight, 32 of narrow words
     const uint32_t slots = (uint32_t)(HALVES ? s.pairs / V : 2 * s.pairs / V);
     s.head_groups = (s.heads + U - 1) / U;
-    const uint64_t most = (uint64_t)slots * s.head_groups;
-    if (most > (1u << 20)) return cudaErrorInvalidValue;
-    const uint32_t per_token = (uint32_t)most;
+    // at most 256 places and 65,536 heads: 2^22 threads of a token, so 2^14 blocks of it and divisions of up to 2^30
+    const uint32_t per_token = slots * s.head_groups;
     s.by_slots = divisor(slots);
     s.by_token = divisor(per_token);
     uint32_t threads, rows = 1; // blocks of 160 threads or a little more (256: 7 % slower on 65,536 tokens): whole tokens, or a part of one

@@ -38,3 +38,20 @@ def test_axes_that_the_positions_lack_become_nan(sa, layout, dtype):
         assert not torch.isnan(x[:, :, q + kv:]).any() and not torch.isnan(x[..., 2 * sum(pairs):]).any()
         want[torch.isnan(x)] = float("nan")
         close(x, want, bound)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "halves"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_heads_in_narrow_words(sa, layout, dtype):
+    """2.6 million places and groups of heads of a token (65536 heads of 256 pairs are 4.2 million): more blocks for a token than
+    1 << 20 threads fill."""
+    q, kv, head, pairs = 40000, 1000, 511, (100, 155)
+    x = randn(1, 2, q + 2 * kv, head, seed=4, dtype=dtype)
+    before = x.clone()
+    places = torch.tensor([[[3, 4000]], [[-7, 99999]]], device="cuda")
+    sa.rope_axes_forward(x, places, sa.rope_axes_spectrum(pairs), q, kv, layout)
+    for heads in (slice(0, 700), slice(20000, 20500), slice(q + kv - 500, q + kv)):
+        part = before[:, :, heads].double()
+        want, bound = ref.rope(part, places, pairs, 10000.0, "own", part.shape[2], 0, layout)
+        close(x[:, :, heads], want, bound)
+    assert torch.equal(x[:, :, q + kv:], before[:, :, q + kv:]) and torch.equal(x[..., 510:], before[..., 510:])

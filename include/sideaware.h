@@ -156,8 +156,8 @@ sideaware_status_t sideaware_silu_mul_bf16(void* out, const void* a, const void*
 
 /* Rotary positions with several axes (time, height, width, ...), in place on packed [B, T, Nq + 2*Nkv, HS]: pair i of
  * every Q and K head is turned by pos[axis(i)][b][t] * f(i).  V heads and the elements of a head behind the first
- * 2*pairs are not touched.  Positions may be negative and need no table; f(i) / 2 pi is held to 2^-62 of a turn, so the angle is off by
- * at most (|pos| * 2^-62 + 2^-32) turns.  The positions have as many axes as the spectrum was made with; pairs
+ * 2*pairs are not touched.  Positions may be negative and need no table; f(i) / 2 pi is held to 2^-62 of a turn (theta below 1:
+ * to 2^-62 / theta), so the angle is off by at most that times |pos|, and by 2^-26 turns from fp32 (4 * 2^-24 of cos and sin in all).  The positions have as many axes as the spectrum was made with; pairs
  * whose axis they lack become NaN, neighbouring pairs possibly with them. */
 #define SIDEAWARE_ROPE_MAX_AXES 8
 #define SIDEAWARE_ROPE_MAX_PAIRS 256

@@ -5,9 +5,9 @@
 //
 // Angles: the spectrum holds f(i) / 2 pi as a 61-bit binary fraction of a turn (the low three bits name the axis), so the
 // integer product with the position, modulo 2^64, is the fraction of a turn without a rounding of its own: no table, and an
-// error of |position| 2^-62 turns, so that position 10^6 is as accurate as position 1.  Its upper 32 bits are kept.  The
-// nearest quarter turn is split off in integers and what is left, at most an eighth of a turn, goes through Taylor
-// polynomials (truncation below 2e-9).
+// error of |position| 2^-62 turns (theta >= 1), so that position 10^6 is as accurate as position 1.  Its upper 32 bits are kept.
+// The nearest quarter turn is split off in integers and what is left, at most an eighth of a turn, becomes an fp32 angle (off by
+// 2^-26.3 turns, from the conversion, the constant and the product) for Taylor polynomials (truncation below 2e-9).
 //
 // Bound: HBM, each turned element is read once and written once.  A thread has one place in the head (its cos and sin
 // are computed once) and several heads of one token in flight.

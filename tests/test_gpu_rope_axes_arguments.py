@@ -55,3 +55,27 @@ def test_many_heads_in_narrow_words(sa, layout, dtype):
         want, bound = ref.rope(part, places, pairs, 10000.0, "own", part.shape[2], 0, layout)
         close(x[:, :, heads], want, bound)
     assert torch.equal(x[:, :, q + kv:], before[:, :, q + kv:]) and torch.equal(x[..., 510:], before[..., 510:])
+
+
+@pytest.mark.parametrize("theta", [1.0, 10000.0, 0.25])
+@pytest.mark.parametrize("name", ["rope_axes_forward", "rope_axes_backward"])
+def test_angles_of_near_and_far_positions(sa, name, theta):
+    """Pairs (1, 0) turn to (cos, sin), the angle to |position| 2^-62 max(1, 1 / theta) + 2^-26 turns as documented.  Beside it an
+    evaluation of cos and sin: a rounding of the result, 2^-24 for the polynomial's own roundings, 2e-9 for its truncation.  The
+    angle itself is worked out in 60 digits."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 60
+    two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+    pairs, places = 8, [0, 1, -1, 17, 1000, 54321, -123457, 10 ** 6 + 1, 2 ** 31 - 1, -2 ** 31, 2 ** 36 + 5, -2 ** 40 - 1, 3 * 10 ** 13]
+    x = torch.zeros(1, len(places), 1, 2 * pairs, device="cuda")
+    x[..., :pairs] = 1.0
+    positions = torch.tensor(places, device="cuda").view(1, 1, -1)
+    getattr(sa, name)(x, positions, sa.rope_axes_spectrum((pairs,), theta), 1, 0, "halves")
+    for t, place in enumerate(places):
+        for i in range(pairs):
+            turns = place * Decimal(theta) ** (Decimal(-i) / pairs) / two_pi
+            angle = float((turns - turns.to_integral_value()) * two_pi) * (1 if name == "rope_axes_forward" else -1)
+            limit = float(two_pi) * (abs(place) * 2.0 ** -62 * max(1.0, 1.0 / theta) + 2.0 ** -26) + 2 * 2.0 ** -24 + 2e-9
+            want = torch.tensor([angle], dtype=torch.float64)
+            assert abs(float(x[0, t, 0, i]) - float(want.cos())) <= limit, (place, i)
+            assert abs(float(x[0, t, 0, pairs + i]) - float(want.sin())) <= limit, (place, i)

@@ -323,8 +323,8 @@ class SideAware:
         import torch
         B, T, H, HS = qkv.shape
         # the C ABI has 32-bit sizes, and ctypes would cut off what does not fit; negative ones are refused as well
-        assert (B | T | H | HS | n_q_heads | n_kv_heads | spectrum.numel() | positions.shape[0]) >> 31 == 0, "sizes must be below 2^31"
-        axes = positions.shape[0]
+        pairs, axes = spectrum.numel(), positions.shape[0]
+        assert (B | T | H | HS | n_q_heads | n_kv_heads | pairs | axes) >> 31 == 0, "sizes must be below 2^31"
         assert getattr(spectrum, "rope_axes", axes) == axes, "positions must have the axes that the spectrum was made with"
         device = qkv.get_device()
         assert device >= 0 and positions.get_device() == device and spectrum.get_device() == device, "all tensors must be on one CUDA device"
@@ -335,7 +335,7 @@ class SideAware:
         assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
         assert spectrum.dim() == 1 and spectrum.dtype == torch.int64 and spectrum.is_contiguous(), "spectrum must be int64 [pairs]"
         assert layout in _ROPE_LAYOUTS, f"layout must be one of {sorted(_ROPE_LAYOUTS)}"
-        shape = _binding.RopeAxes(B, T, n_q_heads, n_kv_heads, HS, spectrum.shape[0], axes, _ROPE_LAYOUTS[layout], _dtype_code(qkv.dtype),
+        shape = _binding.RopeAxes(B, T, n_q_heads, n_kv_heads, HS, pairs, axes, _ROPE_LAYOUTS[layout], _dtype_code(qkv.dtype),
                                   1 if positions.dtype == torch.int64 else 0, sb, st, *positions.stride())
         self._done(call(qkv.data_ptr(), positions.data_ptr(), spectrum.data_ptr(), ctypes.byref(shape), device, _current_stream(device)), what)
 

@@ -20,14 +20,14 @@
 //    in its shared memory at a time and goes on to the next ones, which are already on their way.
 //
 // Bound and measured on a B200 (device time of a call, three sets of inputs in turn):
-//  * resident: the phases of a block follow one another, and each moves about 4 TB/s alone.  8 x 4096 x 320 bf16: 16.7 us (6.4
+//  * resident: the phases of a block follow one another, and each moves about 4 TB/s alone.  8 x 4096 x 320 bf16: 17.1 us (6.4
 //    at the copy's rate), of 31,000 cycles 12,000 are for the rows to arrive, 5,000 for the statistics to go around and
-//    11,500 for SiLU and the stores (without SiLU: 1.4 us less).  Backward the activation's derivative is worked out twice, 32
-//    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.2 us.
-//  * streamed: HBM.  2 x 262144 x 128 bf16: 74.5 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
+//    11,500 for SiLU and the stores (without SiLU: 1.6 us less).  Backward the activation's derivative is worked out twice, 32
+//    operations of the special-function unit for 8 elements: 8 x 1024 x 640 fp16 17.5 us.
+//  * streamed: HBM.  2 x 262144 x 128 bf16: 75.6 us, 29 us for reading x (a plain sum of as many bytes takes as long) and 41
 //    us for the copy-like second pass.
-//  * packed: instructions, 190 of a warp for a word of each lane forward and 560 backward.  16384 x 1 x 2048 bf16: 45 us
-//    and 118 us (resident: 580 and 1080); 1 x 64 x 1280 bf16: 4.0 us, which is latency (resident 5.1).
+//  * packed: instructions, 190 of a warp for a word of each lane forward and 550 backward.  16384 x 1 x 2048 bf16: 45 us
+//    and 117 us (resident: 580 and 1080); 1 x 64 x 1280 bf16: 4.1 us, which is latency (resident 5.1).
 #include <cooperative_groups.h>
 
 #include <algorithm>
